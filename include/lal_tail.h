@@ -6,7 +6,7 @@
  * int8, contract it with the per-row-scaled int8 LM head, apply the
  * repetition penalty, then top-k select, softmax with temperature, draw.
  *
- * Two layers are exported, both plain C: host pointers, sizes, int status.
+ * Three layers are exported, all plain C: pointers, sizes, int status.
  *
  *  1. Drop-ins.  The functions the reference defines as static inline in
  *     runtime/lal_q8_kernel.h and runtime/lal_sampling.h, with the same names
@@ -24,6 +24,9 @@
  *     and returns B token ids, in one kernel per step.  Multi-GPU contexts
  *     each own a contiguous vocab slice and merge the per-slice top-k
  *     candidates across GPUs.
+ *
+ *  3. Layer operators on device memory: the norm, the 4-bit products and the
+ *     activation of the layers before the tail, in its 8-bit form.
  *
  * Every lal_tail_* function returns LAL_TAIL_OK (0) or an error code;
  * lal_tail_last_error() gives the calling thread's last message.
@@ -354,6 +357,97 @@ int lal_tail_debug_phase_read(lal_tail *t, unsigned long long *out, int cap, int
 
 /* Glibc-exact expf as the device computes it (test hook). */
 int lal_tail_debug_expf(const float *x, float *y, int n);
+
+/* ======================================================================
+ * 3. Layer operators on device memory
+ *
+ * What a layer computes around its products, in the form that the tail uses:
+ * activations as 8-bit rows with one fp32 scale each (as
+ * lal_quantize_x_int8 makes them), weights in 4 bits.  One MLP block of a
+ * decode step, into the tail:
+ *
+ *   lal_tail_add_rms_norm_q8  x + residual -> h, and its norm in 8 bits
+ *   lal_tail_q4_matvec        gate and up
+ *   lal_tail_swiglu_q8        silu(gate) * up in 8 bits
+ *   lal_tail_q4_matvec        down; the next norm adds h to it
+ *   lal_tail_step_device      (lal_tail_set_final_norm) on the last h
+ *
+ * All pointers named d_* are device memory of one device, which need not be
+ * the current one; host memory is refused.  Strides count elements from one
+ * row to the next and are at least the row's length; rows need no alignment
+ * beyond their type's.  Each call enqueues its work on `stream` (a
+ * cudaStream_t of that device; NULL = its legacy default stream) and returns;
+ * it allocates nothing, keeps nothing, shares no workspace, and can be
+ * captured.  Zero rows or streams: nothing is done.  Only the rows and columns
+ * named are written, and no output may overlap another buffer of the call,
+ * except where a call says so.  A row's results do not depend on what the
+ * other rows or streams of a call hold, and are the same in every run. */
+#define LAL_TAIL_F32  0
+#define LAL_TAIL_BF16 1
+#define LAL_TAIL_F16  2
+
+/* h = x + residual, rounded to its type, and the RMSNorm of h as 8-bit rows:
+ *   v_i   = h_i * norm_w_i / sqrt(mean(h^2) + eps)
+ *   q_i   = rint(127 v_i / max|v|) (ties to even), scale = max|v| / 127
+ * x, residual and h are [rows, n_embd] of `dtype` (LAL_TAIL_F32, _BF16,
+ * _F16), norm_w is fp32.  The norm is taken of the rounded h, in 64 bits where
+ * it decides a q.  d_residual may be NULL (h = x); d_h may be NULL then (h is
+ * not stored).  d_h may be d_x or d_residual, with the same stride.  A row
+ * whose values are all zero gets scale 0 and q 0; a row with a value that is
+ * not finite, or whose max|v| is above fp32's range, gets scale NaN and q 0.
+ * (qwen7b_server.c:820 and its per-layer norms at :761-817; the quantizer
+ * differs from lal_quantize_x_int8 in rounding 127 v / max once, and in having
+ * no lower limit on the scale.) */
+int lal_tail_add_rms_norm_q8(const void *d_x, int64_t x_stride, const void *d_residual,
+                             int64_t residual_stride, void *d_h, int64_t h_stride, int dtype,
+                             const float *d_norm_w, float eps, int rows, int n_embd, int8_t *d_q,
+                             int64_t q_stride, float *d_scale, void *stream);
+/* The same 8-bit rows of v_i = gate_i / (1 + exp(-gate_i)) * up_i; gate and up
+ * are [rows, n] of `dtype` and may be columns of one buffer (the SwiGLU of the
+ * server's layers, qwen7b_server.c:761-817). */
+int lal_tail_swiglu_q8(const void *d_gate, int64_t gate_stride, const void *d_up, int64_t up_stride,
+                       int dtype, int rows, int n, int8_t *d_q, int64_t q_stride, float *d_scale,
+                       void *stream);
+
+/* Weights [rows, cols] in 4 bits, in memory of the caller's.
+ *   d_q      [rows][LAL_TAIL_Q4_ROW_BYTES(cols)], aligned to 16 bytes: blocks
+ *            of 32 columns, 16 bytes each; byte j of a block holds column j in
+ *            its low half and column j + 16 in its high half (what a block
+ *            holds for columns >= cols is not used)
+ *   d_scale  [rows][LAL_TAIL_Q4_GROUPS(cols, group)] IEEE f16
+ *   d_min    the same, or NULL
+ *   group    32, 64 or 128 columns of a row
+ * With d_min NULL a weight is scale * (q - 8), else scale * q + min. */
+typedef struct {
+    uint8_t *d_q;
+    uint16_t *d_scale;
+    uint16_t *d_min;
+    int rows, cols, group;
+} lal_tail_q4;
+#define LAL_TAIL_Q4_ROW_BYTES(cols) (((size_t)(cols) + 31) / 32 * 16)
+#define LAL_TAIL_Q4_GROUPS(cols, group) (((size_t)(cols) + (group) - 1) / (group))
+#define LAL_TAIL_Q4_MAX_STREAMS 256
+/* Quantizes d_w [w->rows, w->cols] of `dtype` into w's buffers (beside
+ * lal_quantize_q8_per_row, runtime/lal_q8_kernel.h:357).  Without a minimum:
+ * scale = max|w| / 7 of the group, q = rint(w / scale) + 8.  With one: min =
+ * the group's smallest value, scale = (its largest - min) / 15, q = rint((w -
+ * min) / scale).  Scales are rounded up to f16 and minima down, so no weight
+ * is clamped; q is taken with the rounded ones, as in 64 bits (ties to
+ * even).  A group with a value that is not finite, or too large for an f16
+ * scale, gets scale (and minimum) NaN. */
+int lal_tail_quantize_q4(const lal_tail_q4 *w, const void *d_w, int64_t w_stride, int dtype,
+                         void *stream);
+/* The weights' values [w->rows, w->cols] in `dtype`, computed in fp32. */
+int lal_tail_dequantize_q4(const lal_tail_q4 *w, void *d_w, int64_t w_stride, int dtype, void *stream);
+/* y[b, r] = d_scale_x[b] * sum over columns c of xq[b, c] * weight[r, c], for
+ * n_streams (at most LAL_TAIL_Q4_MAX_STREAMS) 8-bit vectors; y is [n_streams,
+ * w->rows] of `dtype`.  The dots of 32 columns are exact integers, their
+ * scaled sum is held in fp32.  xq may hold -128.  (Beside
+ * lal_lm_head_int8_range, runtime/lal_q8_kernel.h:463; the 4-bit products of
+ * the server's layers.) */
+int lal_tail_q4_matvec(const lal_tail_q4 *w, const int8_t *d_xq, int64_t xq_stride,
+                       const float *d_scale_x, int n_streams, void *d_y, int64_t y_stride, int dtype,
+                       void *stream);
 
 #ifdef __cplusplus
 }

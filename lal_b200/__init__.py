@@ -13,6 +13,10 @@ the path, with the reference's names:
   filter hook of qwen7b_server.c:175-186)
 * ``DecodeTail``           the fused tail replacing qwen7b_server.c:829-850
 
+The layer operators work on device memory (addresses as integers, as
+``DecodeTail.step_device`` takes them): ``add_rms_norm_q8``, ``swiglu_q8`` and
+the 4-bit weights ``Q4Weights`` with ``quantize``, ``dequantize``, ``matvec``.
+
 Everything computes on the GPU.  There is no CPU fallback: importing works
 without a GPU (so the library can be inspected), but every compute call
 raises ``LalTailError`` when the CUDA library or a GPU is unavailable.
@@ -31,6 +35,10 @@ LIB_PATH = os.path.join(HERE, "liblal_tail.so")
 LAL_SAMPLER_LIBRARY = 0
 LAL_SAMPLER_SERVER = 1
 LAL_SAMPLER_GPT2 = 2
+LAL_TAIL_F32 = 0
+LAL_TAIL_BF16 = 1
+LAL_TAIL_F16 = 2
+LAL_TAIL_Q4_MAX_STREAMS = 256
 
 ERRORS = {0: "OK", 1: "ERR_ARG", 2: "ERR_CUDA", 3: "ERR_NOMEM", 4: "ERR_TIMEOUT",
           5: "ERR_CAPACITY", 6: "ERR_STATE", 7: "ERR_COMM", 8: "ERR_UNSUPPORTED"}
@@ -66,6 +74,12 @@ class Gpq8Tensor(C.Structure):
                 ("scale_offset", C.c_uint64)]
 
 
+class Q4Desc(C.Structure):
+    """Mirror of ``lal_tail_q4`` (include/lal_tail.h)."""
+    _fields_ = [("d_q", C.c_void_p), ("d_scale", C.c_void_p), ("d_min", C.c_void_p),
+                ("rows", C.c_int), ("cols", C.c_int), ("group", C.c_int)]
+
+
 class RecentTokens(C.Structure):
     """Mirror of LalRecentTokens (runtime/lal_sampling.h:128-131)."""
     _fields_ = [("tokens", C.c_int * 256), ("n", C.c_int)]
@@ -82,6 +96,7 @@ _u8p = np.ctypeslib.ndpointer(np.uint8, flags="C_CONTIGUOUS")
 _i32p = np.ctypeslib.ndpointer(np.int32, flags="C_CONTIGUOUS")
 _vp = C.c_void_p
 _ip = C.c_int
+_i64 = C.c_int64
 _fp = C.c_float
 
 # name -> (restype, argtypes); every symbol of include/lal_tail.h
@@ -143,6 +158,12 @@ SIGNATURES = {
     "lal_tail_get_stream": (C.c_int, [_vp, C.POINTER(_vp)]),
     "lal_tail_set_timing": (C.c_int, [_vp, _ip]),
     "lal_tail_kernel_time": (C.c_int, [_vp, C.POINTER(C.c_double), C.POINTER(C.c_int)]),
+    "lal_tail_add_rms_norm_q8": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _ip, _vp, _fp, _ip, _ip,
+                                           _vp, _i64, _vp, _vp]),
+    "lal_tail_swiglu_q8": (C.c_int, [_vp, _i64, _vp, _i64, _ip, _ip, _ip, _vp, _i64, _vp, _vp]),
+    "lal_tail_quantize_q4": (C.c_int, [_vp, _vp, _i64, _ip, _vp]),
+    "lal_tail_dequantize_q4": (C.c_int, [_vp, _vp, _i64, _ip, _vp]),
+    "lal_tail_q4_matvec": (C.c_int, [_vp, _vp, _i64, _vp, _ip, _vp, _i64, _ip, _vp]),
     "lal_tail_debug_expf": (C.c_int, [_f32p, _f32p, _ip]),
     "lal_tail_debug_phases": (C.c_int, [_vp, _ip]),
     "lal_tail_debug_phase_read": (C.c_int, [_vp, _vp, _ip, C.POINTER(C.c_int)]),
@@ -273,6 +294,80 @@ def debug_expf(x: np.ndarray) -> np.ndarray:
     y = np.empty_like(x)
     _check(lib().lal_tail_debug_expf(x, y, x.size))
     return y
+
+
+# ---- layer operators on device memory ------------------------------------------------
+
+def add_rms_norm_q8(d_x: int, d_residual: Optional[int], d_h: Optional[int], d_norm_w: int,
+                    eps: float, rows: int, n_embd: int, d_q: int, d_scale: int,
+                    dtype: int = LAL_TAIL_F32, x_stride: Optional[int] = None,
+                    residual_stride: Optional[int] = None, h_stride: Optional[int] = None,
+                    q_stride: Optional[int] = None, stream: Optional[int] = None):
+    """h = x + residual and the RMSNorm of h as 8-bit rows with a scale each
+    (lal_tail_add_rms_norm_q8).  Strides default to n_embd."""
+    rc = lib().lal_tail_add_rms_norm_q8(
+        d_x, n_embd if x_stride is None else x_stride,
+        d_residual, n_embd if residual_stride is None else residual_stride,
+        d_h, n_embd if h_stride is None else h_stride, dtype, d_norm_w, eps, rows, n_embd,
+        d_q, n_embd if q_stride is None else q_stride, d_scale, stream)
+    if rc:
+        _check(rc)
+
+
+def swiglu_q8(d_gate: int, d_up: int, rows: int, n: int, d_q: int, d_scale: int,
+              dtype: int = LAL_TAIL_F32, gate_stride: Optional[int] = None,
+              up_stride: Optional[int] = None, q_stride: Optional[int] = None,
+              stream: Optional[int] = None):
+    """silu(gate) * up as 8-bit rows with a scale each (lal_tail_swiglu_q8).
+    Strides default to n."""
+    rc = lib().lal_tail_swiglu_q8(
+        d_gate, n if gate_stride is None else gate_stride, d_up, n if up_stride is None else up_stride,
+        dtype, rows, n, d_q, n if q_stride is None else q_stride, d_scale, stream)
+    if rc:
+        _check(rc)
+
+
+class Q4Weights:
+    """Weights [rows, cols] in 4 bits with a scale per group of columns, in
+    device memory of the caller's: d_q [rows, row_bytes(cols)] uint8, d_scale
+    and (or None) d_min [rows, groups(cols, group)] f16."""
+
+    def __init__(self, d_q: int, d_scale: int, d_min: Optional[int], rows: int, cols: int,
+                 group: int = 32):
+        self.desc = Q4Desc(d_q, d_scale, d_min, rows, cols, group)
+        self._ref = C.addressof(self.desc)
+
+    @staticmethod
+    def row_bytes(cols: int) -> int:
+        return (cols + 31) // 32 * 16
+
+    @staticmethod
+    def groups(cols: int, group: int) -> int:
+        return (cols + group - 1) // group
+
+    def quantize(self, d_w: int, dtype: int = LAL_TAIL_F32, w_stride: Optional[int] = None,
+                 stream: Optional[int] = None):
+        """Fill the buffers from rows of `dtype` (lal_tail_quantize_q4)."""
+        _check(lib().lal_tail_quantize_q4(
+            self._ref, d_w, self.desc.cols if w_stride is None else w_stride, dtype, stream))
+
+    def dequantize(self, d_w: int, dtype: int = LAL_TAIL_F32, w_stride: Optional[int] = None,
+                   stream: Optional[int] = None):
+        """The weights' values in `dtype` (lal_tail_dequantize_q4)."""
+        _check(lib().lal_tail_dequantize_q4(
+            self._ref, d_w, self.desc.cols if w_stride is None else w_stride, dtype, stream))
+
+    def matvec(self, d_xq: int, d_scale_x: int, n_streams: int, d_y: int, dtype: int = LAL_TAIL_F32,
+               xq_stride: Optional[int] = None, y_stride: Optional[int] = None,
+               stream: Optional[int] = None):
+        """y = scale_x * (xq times the weights) for n_streams 8-bit vectors
+        (lal_tail_q4_matvec)."""
+        d = self.desc
+        rc = lib().lal_tail_q4_matvec(
+            self._ref, d_xq, d.cols if xq_stride is None else xq_stride, d_scale_x, n_streams,
+            d_y, d.rows if y_stride is None else y_stride, dtype, stream)
+        if rc:
+            _check(rc)
 
 
 # ---- the fused decode tail -----------------------------------------------------------

@@ -1,0 +1,114 @@
+/*
+ * tail_layer.h -- what the layer operators (tail_q8.cu, tail_q4.cu) share:
+ * their types, the checks of their device pointers and the device that a call
+ * runs on.  Not installed.
+ */
+#pragma once
+
+#include "../../include/lal_tail.h"
+#include "tail_internal.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+namespace lal {
+
+inline int layer_fail(int code, const char *fmt, ...) {
+    char buf[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return set_error(code, buf);
+}
+
+inline int dtype_size(int dtype) {
+    return dtype == LAL_TAIL_F32 ? 4 : dtype == LAL_TAIL_BF16 || dtype == LAL_TAIL_F16 ? 2 : 0;
+}
+
+/* The bytes that `rows` rows of `n` elements, `stride` elements apart, span. */
+struct Span {
+    uintptr_t lo = 0, hi = 0;
+    Span() {}
+    Span(const void *p, long long rows, long long n, long long stride, int size) {
+        if (p == nullptr || rows < 1) return;
+        lo = (uintptr_t)p;
+        hi = lo + (uintptr_t)((rows - 1) * stride + n) * size;
+    }
+    bool meets(const Span &o) const { return lo < o.hi && o.lo < hi; }
+};
+
+/* The device whose memory p is; host memory is refused here, before a kernel
+ * could fault on it. */
+inline int pointer_device(const char *op, const char *what, const void *p, int *dev) {
+    cudaPointerAttributes a;
+    const cudaError_t e = cudaPointerGetAttributes(&a, p);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return layer_fail(LAL_TAIL_ERR_CUDA, "%s: %s: %s", op, what, cudaGetErrorString(e));
+    }
+    if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged)
+        return layer_fail(LAL_TAIL_ERR_ARG, "%s: %s is not device memory", op, what);
+    *dev = a.device;
+    return LAL_TAIL_OK;
+}
+
+/* Makes the device of a call's memory current while the call launches, and
+ * the caller's device again after it. */
+class CallDevice {
+    int before_ = -1;
+
+  public:
+    /* every pointer that is not null has to be memory of one device */
+    int enter(const char *op, const char *const *names, const void *const *ptrs, int n) {
+        int dev = -1;
+        for (int i = 0; i < n; ++i) {
+            if (ptrs[i] == nullptr) continue;
+            int d = -1;
+            const int rc = pointer_device(op, names[i], ptrs[i], &d);
+            if (rc != LAL_TAIL_OK) return rc;
+            if (dev >= 0 && d != dev)
+                return layer_fail(LAL_TAIL_ERR_ARG, "%s: %s is on device %d, other memory on device %d",
+                                  op, names[i], d, dev);
+            dev = d;
+        }
+        int now = -1;
+        cudaError_t e = cudaGetDevice(&now);
+        if (e == cudaSuccess && now != dev) {
+            e = cudaSetDevice(dev);
+            if (e == cudaSuccess) before_ = now;
+        }
+        if (e != cudaSuccess) {
+            (void)cudaGetLastError();
+            return layer_fail(LAL_TAIL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+        }
+        return LAL_TAIL_OK;
+    }
+    ~CallDevice() {
+        if (before_ >= 0) cudaSetDevice(before_);
+    }
+};
+
+inline int launched(const char *op, cudaError_t e) {
+    if (e == cudaSuccess) return LAL_TAIL_OK;
+    (void)cudaGetLastError(); /* reported here; leave no stale error behind */
+    return layer_fail(LAL_TAIL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+}
+
+#if defined(__CUDACC__)
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+#endif
+
+}  // namespace lal
