@@ -60,7 +60,7 @@ inline int pointer_device(const char *op, const char *what, const void *p, int *
 /* Makes the device of a call's memory current while the call launches, and
  * the caller's device again after it. */
 class CallDevice {
-    int before_ = -1;
+    int before_ = -1, dev_ = -1;
 
   public:
     /* every pointer that is not null has to be memory of one device */
@@ -86,7 +86,16 @@ class CallDevice {
             (void)cudaGetLastError();
             return layer_fail(LAL_TAIL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
         }
+        dev_ = dev;
         return LAL_TAIL_OK;
+    }
+    int num_sms() const {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev_) != cudaSuccess || n < 1) {
+            (void)cudaGetLastError();
+            n = 148;
+        }
+        return n;
     }
     ~CallDevice() {
         if (before_ >= 0) cudaSetDevice(before_);

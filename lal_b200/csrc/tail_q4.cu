@@ -14,6 +14,9 @@
  */
 #include "tail_layer.h"
 
+#include <algorithm>
+#include <type_traits>
+
 using namespace lal;
 
 namespace {
@@ -147,70 +150,252 @@ struct MatvecParams {
     int streams, rows, cols, group;
     void *y;
     long long y_stride;
+    int dtype;
 };
 
-/* four consecutive columns of a vector, zeros behind its end */
-__device__ __forceinline__ int x_word(const int8_t *x, int c, int cols) {
-    uint32_t v = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (c + j < cols) v |= (uint32_t)(uint8_t)x[c + j] << (8 * j);
-    return (int)v;
+/* ---- up to eight streams: mma.sync m16n8k32 on int8 ----
+ *
+ * A warp takes 16 rows and every kWarpsK-th stage of 256 columns; the rows'
+ * 4-bit words and the vectors go through a ring of shared memory of its own
+ * (cp.async, no barrier of the CTA until the warps' sums are joined).  A
+ * block's word t of row g, shifted and masked, is that lane's part of the A
+ * operand for columns 4t.. and 16 + 4t..: q - 8 in the upper half of a byte is
+ * 16 (q - 8) as int8, so the dots come out 16 times too large and the scales
+ * carry 1/16.  The dots of a group are exact int32 (below 2^24), and are
+ * scaled and added in fp32.  With a minimum, w = s (q - 8) + (8 s + m): a
+ * second product with rows of 16 gives 16 times the sums of the vectors. */
+constexpr int kMmaWarps = 8;
+constexpr int kMmaStreams = 8;
+constexpr int kStageBlocks = 8;               /* 256 columns */
+constexpr int kStageA = 16 * (kStageBlocks * 16 + 16); /* rows 16 bytes apart mod 128: no bank conflicts */
+constexpr int kStageXRow = kStageBlocks * 32 + 16;
+constexpr int kMmaSmem = 108 * 1024 + 512; /* two CTAs an SM, with their static 4 KB */
+static_assert(kMmaWarps * 3 * (kStageA + 8 * kStageXRow) <= kMmaSmem, "five to eight streams, three stages");
+static_assert(kMmaWarps * 4 * (kStageA + 4 * kStageXRow) <= kMmaSmem, "up to four streams, four stages");
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+/* 16 (or 4) bytes to shared memory, the last 16 - n of them zeros */
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async16_l1(uint32_t dst, const void *src, int n) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-/* A warp takes a row and up to kB streams; a lane takes every 32nd block of
- * the row.  The dots of a block are exact integers; their scaled sum is in
- * 32-bit floats. */
-template <typename T, int kB, bool kMin>
-__global__ void __launch_bounds__(256) q4_matvec_kernel(const MatvecParams p) {
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (row >= p.rows) return;
-    const int b0 = blockIdx.y * kB;
-    const int blocks = q4_blocks(p.cols), groups = (p.cols + p.group - 1) / p.group;
-    const uint4 *q = (const uint4 *)p.q + (size_t)row * blocks;
-    float acc[kB] = {};
-    for (int k = lane; k < blocks; k += 32) {
-        const uint4 v = __ldg(q + k);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        const size_t g = (size_t)row * groups + k * kQ4Block / p.group;
-        const float s = __half2float(p.scale[g]);
-        const float m = kMin ? __half2float(p.min[g]) : __fmul_rn(s, -8.0f);
+/* 16 columns (c0 ..) of a vector's row to shared memory, zeros behind its end.
+ * Rows that are not aligned to 16 bytes are read as aligned words and shifted,
+ * byte by byte at the row's ends (no byte outside the row is read). */
+__device__ __forceinline__ void stage_x16(uint32_t dst, const int8_t *row, int c0, int cols) {
+    const int n = max(0, min(16, cols - c0));
+    const int8_t *src = row + (n > 0 ? c0 : 0);
+    const unsigned off = (unsigned)((uintptr_t)src & 15);
+    if (off == 0 && n > 0) {
+        cp_async16_l1(dst, src, n);
+        return;
+    }
+    uint32_t v[4] = {0, 0, 0, 0};
+    const unsigned o4 = off & 3;
+    if (c0 >= 4 && c0 + 20 <= cols) {
+        const uint32_t *w = (const uint32_t *)(src - o4);
+        uint32_t a = __ldg(w);
 #pragma unroll
-        for (int b = 0; b < kB; ++b) {
-            if (b0 + b >= p.streams) break;
-            const int8_t *x = p.x + (size_t)(b0 + b) * p.x_stride;
-            int dot = 0, sum = 0;
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t b = __ldg(w + i + 1);
+            v[i] = __funnelshift_r(a, b, 8 * o4);
+            a = b;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < n) v[i / 4] |= (uint32_t)(uint8_t)__ldg(src + i) << (8 * (i % 4));
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                 : "memory");
+}
+
+__device__ __forceinline__ void store_y(const MatvecParams &p, int b, int row, float v) {
+    const size_t at = (size_t)b * p.y_stride + row;
+    v = __fmul_rn(__ldg(p.sx + b), v);
+    if (p.dtype == LAL_TAIL_F32)
+        ((float *)p.y)[at] = v;
+    else if (p.dtype == LAL_TAIL_BF16)
+        ((__nv_bfloat16 *)p.y)[at] = __float2bfloat16_rn(v);
+    else
+        ((__half *)p.y)[at] = __float2half_rn(v);
+}
+
+template <int kGroup, bool kMin, int kDepth>
+__global__ void __launch_bounds__(32 * kMmaWarps, 2) q4_mma_kernel(const MatvecParams p, int warps_k) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float part[kMmaWarps][16 * kMmaStreams];
+    constexpr int kPer = kGroup / kQ4Block;             /* blocks of a group */
+    constexpr int kGroups = kStageBlocks / kPer;        /* groups of a stage */
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int wk = warp % warps_k;
+    const int row0 = (blockIdx.x * (kMmaWarps / warps_k) + warp / warps_k) * 16;
+    const int b0 = blockIdx.y * kMmaStreams, nx = min(kMmaStreams, p.streams - b0);
+    const int nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
+    const int stages = (nb + kStageBlocks - 1) / kStageBlocks;
+    const int stage_bytes = kStageA + min(kMmaStreams, p.streams) * kStageXRow;
+    const uint32_t ring = smem_u32(smem) + warp * kDepth * stage_bytes;
+
+    auto load = [&](int st, int slot) {
+        const uint32_t a = ring + slot * stage_bytes;
+        const int k0 = st * kStageBlocks;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = (lane >> 3) + 4 * j, k = lane & 7;
+            const bool in = k0 + k < nb;
+            const uint8_t *src = p.q + ((size_t)min(row0 + r, p.rows - 1) * nb + (in ? k0 + k : 0)) * 16;
+            cp_async16(a + r * (kStageBlocks * 16 + 16) + k * 16, src, in ? 16 : 0);
+        }
+        for (int c = lane; c < nx * 16; c += 32)
+            stage_x16(a + kStageA + (c >> 4) * kStageXRow + (c & 15) * 16, p.x + (size_t)(b0 + (c >> 4)) * p.x_stride,
+                      k0 * kQ4Block + (c & 15) * 16, p.cols);
+    };
+    /* lane t holds groups t and t + 4 of a stage of rows g and g + 8: scale, minimum above it */
+    uint32_t sm[2][2] = {}, sm_next[2][2] = {};
+    auto load_scales = [&](int st, uint32_t (&out)[2][2]) {
+#pragma unroll
+        for (int i = 0; i < (kGroups + 3) / 4; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int gr = st * kGroups + t + 4 * i;
+                out[h][i] = 0;
+                if (t + 4 * i < kGroups && gr < groups) {
+                    const size_t at = (size_t)min(row0 + g + 8 * h, p.rows - 1) * groups + gr;
+                    out[h][i] = __ldg((const unsigned short *)p.scale + at);
+                    if (kMin) out[h][i] |= (uint32_t)__ldg((const unsigned short *)p.min + at) << 16;
+                }
+            }
+    };
+
+    float acc[4] = {};
+    const bool live = row0 < p.rows;
+    if (live) {
+        if (wk < stages) load_scales(wk, sm_next);
+#pragma unroll
+        for (int i = 0; i < kDepth - 1; ++i) {
+            if (wk + i * warps_k < stages) load(wk + i * warps_k, i);
+            cp_async_commit();
+        }
+        int slot = 0;
+        const int xg = min(g, nx - 1); /* vectors that are not there: any, their sums are dropped */
+        for (int st = wk; st < stages; st += warps_k) {
+            cp_async_wait<kDepth - 2>();
+            __syncwarp();
+            {
+                const int next = st + (kDepth - 1) * warps_k;
+                if (next < stages) load(next, slot == 0 ? kDepth - 1 : slot - 1);
+                cp_async_commit();
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) sm[h][i] = sm_next[h][i];
+            if (st + warps_k < stages) load_scales(st + warps_k, sm_next);
+            const uint32_t a = ring + slot * stage_bytes + g * (kStageBlocks * 16 + 16) + 4 * t;
+            const uint32_t x = ring + slot * stage_bytes + kStageA + xg * kStageXRow + 4 * t;
+            const int left = nb - st * kStageBlocks; /* blocks from this stage on */
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr) {
+                if (gr * kPer >= left) break;
+                int c[4] = {}, cx[4] = {};
+#pragma unroll
+                for (int k = gr * kPer; k < (gr + 1) * kPer; ++k) {
+                    /* blocks behind the row's end hold zeros in the vectors */
+                    uint32_t w0, w1, x0, x1;
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0) : "r"(a + k * 16));
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1) : "r"(a + 8 * (kStageBlocks * 16 + 16) + k * 16));
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x0) : "r"(x + k * 32));
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x1) : "r"(x + k * 32 + 16));
+                    const uint32_t av[4] = {((w0 << 4) & 0xf0f0f0f0u) ^ 0x80808080u, ((w1 << 4) & 0xf0f0f0f0u) ^ 0x80808080u,
+                                            (w0 & 0xf0f0f0f0u) ^ 0x80808080u, (w1 & 0xf0f0f0f0u) ^ 0x80808080u};
+                    mma_s8(c, av, x0, x1);
+                    if (kMin) {
+                        const uint32_t ones[4] = {0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u};
+                        mma_s8(cx, ones, x0, x1);
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t both = __shfl_sync(0xffffffffu, sm[h][gr / 4], (lane & ~3) | (gr & 3));
+                    const float s = __half2float(__ushort_as_half((unsigned short)both));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        acc[2 * h + i] = fmaf(s * 0.0625f, (float)c[2 * h + i], acc[2 * h + i]);
+                    if (kMin) {
+                        const float m = fmaf(8.0f, s, __half2float(__ushort_as_half((unsigned short)(both >> 16))));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            acc[2 * h + i] = fmaf(m * 0.0625f, (float)cx[i], acc[2 * h + i]);
+                    }
+                }
+            }
+            slot = slot + 1 == kDepth ? 0 : slot + 1;
+        }
+        cp_async_wait<0>();
+    }
+    if (warps_k == 1) {
+        if (live)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int lo = x_word(x, k * kQ4Block + 4 * i, p.cols);
-                const int hi = x_word(x, k * kQ4Block + 16 + 4 * i, p.cols);
-                dot = __dp4a((int)(w[i] & 0x0f0f0f0fu), lo, dot);
-                dot = __dp4a((int)((w[i] >> 4) & 0x0f0f0f0fu), hi, dot);
-                sum = __dp4a(0x01010101, lo, __dp4a(0x01010101, hi, sum));
+                const int row = row0 + g + (i >> 1) * 8, b = 2 * t + (i & 1);
+                if (row < p.rows && b < nx) store_y(p, b0 + b, row, acc[i]);
             }
-            if (kMin)
-                acc[b] = fmaf(m, (float)sum, fmaf(s, (float)dot, acc[b]));
-            else
-                acc[b] = fmaf(s, (float)(dot - 8 * sum), acc[b]);
-        }
+        return;
     }
+    /* the warps of a row tile, in order */
 #pragma unroll
-    for (int b = 0; b < kB; ++b) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) acc[b] += __shfl_xor_sync(0xffffffffu, acc[b], o);
-        if (lane == 0 && b0 + b < p.streams)
-            ((T *)p.y)[(size_t)(b0 + b) * p.y_stride + row] =
-                from_f32<T>(__fmul_rn(p.sx[b0 + b], acc[b]));
+    for (int i = 0; i < 4; ++i) part[warp][(2 * t + (i & 1)) * 16 + g + (i >> 1) * 8] = acc[i];
+    __syncthreads();
+    const int tiles = kMmaWarps / warps_k;
+    for (int i = threadIdx.x; i < tiles * 16 * nx; i += 32 * kMmaWarps) {
+        const int r = i & 15, b = (i >> 4) % nx, tile = (i >> 4) / nx;
+        const int row = (blockIdx.x * tiles + tile) * 16 + r;
+        if (row >= p.rows) continue;
+        float sum = 0.0f;
+        for (int w = 0; w < warps_k; ++w) sum += part[tile * warps_k + w][b * 16 + r];
+        store_y(p, b0 + b, row, sum);
     }
 }
 
-template <typename T, bool kMin> cudaError_t launch_matvec(const MatvecParams &p, cudaStream_t st) {
-    const unsigned gx = (unsigned)((p.rows + 7) / 8);
-    if (p.streams == 1)
-        q4_matvec_kernel<T, 1, kMin><<<dim3(gx, 1), 256, 0, st>>>(p);
-    else
-        q4_matvec_kernel<T, 8, kMin><<<dim3(gx, (p.streams + 7) / 8), 256, 0, st>>>(p);
+template <int kGroup, bool kMin, int kDepth>
+cudaError_t launch_mma(const MatvecParams &p, int num_sms, cudaStream_t st) {
+    /* warps of a row tile: enough that the tiles' warps fill the SMs (16 a SM),
+     * no more than there are stages */
+    const int tiles = (p.rows + 15) / 16, stages = (q4_blocks(p.cols) + kStageBlocks - 1) / kStageBlocks;
+    int wk = 1;
+    while (wk < kMmaWarps && 2 * wk <= stages && (long long)tiles * wk < 16LL * num_sms) wk *= 2;
+    const int smem = kMmaWarps * kDepth * (kStageA + std::min(kMmaStreams, p.streams) * kStageXRow);
+    const void *fn = (const void *)q4_mma_kernel<kGroup, kMin, kDepth>;
+    cudaError_t e = raise_smem(fn, kMmaSmem);
+    if (e != cudaSuccess) return e;
+    const int per = kMmaWarps / wk;
+    q4_mma_kernel<kGroup, kMin, kDepth>
+        <<<dim3((tiles + per - 1) / per, (p.streams + kMmaStreams - 1) / kMmaStreams), 32 * kMmaWarps, smem, st>>>(p, wk);
     return cudaGetLastError();
+}
+
+template <int kGroup, bool kMin> cudaError_t launch_matvec(const MatvecParams &p, int num_sms, cudaStream_t st) {
+    /* two CTAs of at most 110 KB a SM */
+    return p.streams <= 4 ? launch_mma<kGroup, kMin, 4>(p, num_sms, st) : launch_mma<kGroup, kMin, 3>(p, num_sms, st);
+}
+
+template <int kGroup> cudaError_t launch_matvec(const MatvecParams &p, int num_sms, cudaStream_t st) {
+    return p.min != nullptr ? launch_matvec<kGroup, true>(p, num_sms, st) : launch_matvec<kGroup, false>(p, num_sms, st);
 }
 
 /* calls f with the type of `dtype` and the truth of `min` as constants */
@@ -334,10 +519,12 @@ int lal_tail_q4_matvec(const lal_tail_q4 *w, const int8_t *d_xq, int64_t xq_stri
     CallDevice dev;
     if (const int rc = dev.enter(op, names, ptrs, 6)) return rc;
     const MatvecParams p = {d_xq, xq_stride, d_scale_x, w->d_q, (const __half *)w->d_scale,
-                            (const __half *)w->d_min, n_streams, w->rows, w->cols, w->group, d_y, y_stride};
-    return launched(op, by_type(dtype, w->d_min != nullptr, [&](auto t, auto min) {
-        return launch_matvec<decltype(t), decltype(min)::value>(p, (cudaStream_t)stream);
-    }));
+                            (const __half *)w->d_min, n_streams, w->rows, w->cols, w->group, d_y, y_stride, dtype};
+    cudaStream_t st = (cudaStream_t)stream;
+    const int sms = dev.num_sms();
+    return launched(op, w->group == 32   ? launch_matvec<32>(p, sms, st)
+                        : w->group == 64 ? launch_matvec<64>(p, sms, st)
+                                         : launch_matvec<128>(p, sms, st));
 }
 
 }  // extern "C"
