@@ -167,11 +167,13 @@ struct MatvecParams {
 constexpr int kMmaWarps = 8;
 constexpr int kMmaStreams = 8;
 constexpr int kStageBlocks = 8;               /* 256 columns */
-constexpr int kStageA = 16 * (kStageBlocks * 16 + 16); /* rows 16 bytes apart mod 128: no bank conflicts */
-constexpr int kStageXRow = kStageBlocks * 32 + 16;
-constexpr int kMmaSmem = 108 * 1024 + 512; /* two CTAs an SM, with their static 4 KB */
-static_assert(kMmaWarps * 3 * (kStageA + 8 * kStageXRow) <= kMmaSmem, "five to eight streams, three stages");
-static_assert(kMmaWarps * 4 * (kStageA + 4 * kStageXRow) <= kMmaSmem, "up to four streams, four stages");
+constexpr int kStageARow = kStageBlocks * 16; /* block k of row r in place k ^ (r mod 8): no bank conflicts */
+constexpr int kStageA = 16 * kStageARow;
+constexpr int kStageS = 2 * 16 * 2 * kStageBlocks; /* scales and minima, groups of 32 */
+constexpr int kStageXRow = kStageBlocks * 32 + 16; /* rows 16 bytes apart mod 128 */
+constexpr int kMmaSmem = 113 * 1024 - 1024; /* two CTAs an SM */
+static_assert(kMmaWarps * 3 * (kStageA + kStageS + 8 * kStageXRow) <= kMmaSmem, "up to eight streams, three stages");
+static_assert(kMmaWarps * 4 * (kStageA + kStageS + 3 * kStageXRow) <= kMmaSmem, "up to three streams, four stages");
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
     return (uint32_t)__cvta_generic_to_shared(p);
@@ -188,32 +190,31 @@ template <int N> __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                 "{%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-/* 16 columns (c0 ..) of a vector's row to shared memory, zeros behind its end.
- * Rows that are not aligned to 16 bytes are read as aligned words and shifted,
- * byte by byte at the row's ends (no byte outside the row is read). */
-__device__ __forceinline__ void stage_x16(uint32_t dst, const int8_t *row, int c0, int cols) {
+/* n (0 to 16) columns c0 .. of a vector's row to 16 bytes of shared memory,
+ * zeros behind them.  Rows that are not aligned to 16 bytes are read as aligned
+ * words and shifted, byte by byte at the row's ends (no byte outside the row is
+ * read). */
+__device__ __forceinline__ void stage_x16(uint8_t *dst, const int8_t *row, int c0, int cols, bool aligned) {
     const int n = max(0, min(16, cols - c0));
     const int8_t *src = row + (n > 0 ? c0 : 0);
-    const unsigned off = (unsigned)((uintptr_t)src & 15);
-    if (off == 0 && n > 0) {
-        cp_async16_l1(dst, src, n);
+    if (aligned) {
+        cp_async16_l1(smem_u32(dst), src, n);
         return;
     }
     uint32_t v[4] = {0, 0, 0, 0};
-    const unsigned o4 = off & 3;
     if (c0 >= 4 && c0 + 20 <= cols) {
-        const uint32_t *w = (const uint32_t *)(src - o4);
+        const unsigned off = (unsigned)((uintptr_t)src & 3);
+        const uint32_t *w = (const uint32_t *)(src - off);
         uint32_t a = __ldg(w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t b = __ldg(w + i + 1);
-            v[i] = __funnelshift_r(a, b, 8 * o4);
+            v[i] = __funnelshift_r(a, b, 8 * off);
             a = b;
         }
     } else {
@@ -221,8 +222,7 @@ __device__ __forceinline__ void stage_x16(uint32_t dst, const int8_t *row, int c
         for (int i = 0; i < 16; ++i)
             if (i < n) v[i / 4] |= (uint32_t)(uint8_t)__ldg(src + i) << (8 * (i % 4));
     }
-    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
-                 : "memory");
+    *(uint4 *)dst = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 __device__ __forceinline__ void store_y(const MatvecParams &p, int b, int row, float v) {
@@ -239,7 +239,6 @@ __device__ __forceinline__ void store_y(const MatvecParams &p, int b, int row, f
 template <int kGroup, bool kMin, int kDepth>
 __global__ void __launch_bounds__(32 * kMmaWarps, 2) q4_mma_kernel(const MatvecParams p, int warps_k) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float part[kMmaWarps][16 * kMmaStreams];
     constexpr int kPer = kGroup / kQ4Block;             /* blocks of a group */
     constexpr int kGroups = kStageBlocks / kPer;        /* groups of a stage */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -248,44 +247,50 @@ __global__ void __launch_bounds__(32 * kMmaWarps, 2) q4_mma_kernel(const MatvecP
     const int b0 = blockIdx.y * kMmaStreams, nx = min(kMmaStreams, p.streams - b0);
     const int nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
     const int stages = (nb + kStageBlocks - 1) / kStageBlocks;
-    const int stage_bytes = kStageA + min(kMmaStreams, p.streams) * kStageXRow;
-    const uint32_t ring = smem_u32(smem) + warp * kDepth * stage_bytes;
-
-    auto load = [&](int st, int slot) {
-        const uint32_t a = ring + slot * stage_bytes;
-        const int k0 = st * kStageBlocks;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = (lane >> 3) + 4 * j, k = lane & 7;
-            const bool in = k0 + k < nb;
-            const uint8_t *src = p.q + ((size_t)min(row0 + r, p.rows - 1) * nb + (in ? k0 + k : 0)) * 16;
-            cp_async16(a + r * (kStageBlocks * 16 + 16) + k * 16, src, in ? 16 : 0);
-        }
-        for (int c = lane; c < nx * 16; c += 32)
-            stage_x16(a + kStageA + (c >> 4) * kStageXRow + (c & 15) * 16, p.x + (size_t)(b0 + (c >> 4)) * p.x_stride,
-                      k0 * kQ4Block + (c & 15) * 16, p.cols);
-    };
-    /* lane t holds groups t and t + 4 of a stage of rows g and g + 8: scale, minimum above it */
-    uint32_t sm[2][2] = {}, sm_next[2][2] = {};
-    auto load_scales = [&](int st, uint32_t (&out)[2][2]) {
-#pragma unroll
-        for (int i = 0; i < (kGroups + 3) / 4; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int gr = st * kGroups + t + 4 * i;
-                out[h][i] = 0;
-                if (t + 4 * i < kGroups && gr < groups) {
-                    const size_t at = (size_t)min(row0 + g + 8 * h, p.rows - 1) * groups + gr;
-                    out[h][i] = __ldg((const unsigned short *)p.scale + at);
-                    if (kMin) out[h][i] |= (uint32_t)__ldg((const unsigned short *)p.min + at) << 16;
-                }
-            }
-    };
+    const int stage_bytes = kStageA + kStageS + min(kMmaStreams, p.streams) * kStageXRow;
+    uint8_t *ring = smem + warp * kDepth * stage_bytes;
 
     float acc[4] = {};
     const bool live = row0 < p.rows;
     if (live) {
-        if (wk < stages) load_scales(wk, sm_next);
+        /* this lane's share of a stage: four 16-byte blocks of weights, up to four of the vectors */
+        const uint8_t *qsrc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            qsrc[j] = p.q + ((size_t)min(row0 + (lane >> 3) + 4 * j, p.rows - 1) * nb + (lane & 7)) * 16;
+        const uint32_t qdst = (lane >> 3) * kStageARow + ((lane & 7) ^ (lane >> 3)) * 16;
+        const int8_t *xrow = p.x + (size_t)(b0 + min(lane >> 4, nx - 1)) * p.x_stride;
+        const bool x_aligned = (((uintptr_t)p.x | (uintptr_t)p.x_stride) & 15) == 0;
+        /* scales of lane's row, kGroups a stage: one copy where every row's are aligned to it */
+        const unsigned short *ssrc = (const unsigned short *)(lane < 16 ? p.scale : p.min) +
+                                     (size_t)min(row0 + (lane & 15), p.rows - 1) * groups;
+        const bool s_aligned = ((((uintptr_t)p.scale | (kMin ? (uintptr_t)p.min : 0) | (uintptr_t)(groups * 2)) & (2 * kGroups - 1)) == 0);
+        auto load = [&](int st, int slot) {
+            uint8_t *a = ring + slot * stage_bytes;
+            const int k0 = st * kStageBlocks;
+            const bool in = k0 + (lane & 7) < nb;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                cp_async16(smem_u32(a + ((qdst + 4 * j * kStageARow) ^ (j & 1 ? 64 : 0))), in ? qsrc[j] + (size_t)k0 * 16 : p.q, in ? 16 : 0);
+            if (kMin || lane < 16) {
+                /* [16 rows][kGroups] scales, then minima */
+                unsigned short *d = (unsigned short *)(a + kStageA) + lane * kGroups;
+                const int g0 = st * kGroups;
+                if (s_aligned && g0 + kGroups <= groups) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(d)), "l"(ssrc + g0),
+                                 "n"(2 * kGroups)
+                                 : "memory");
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kGroups; ++i)
+                        if (g0 + i < groups) d[i] = __ldg(ssrc + g0 + i);
+                }
+            }
+            const int8_t *xr = xrow;
+            for (int c = lane; c < nx * 16; c += 32, xr += 2 * p.x_stride)
+                stage_x16(a + kStageA + kStageS + (c >> 4) * kStageXRow + (c & 15) * 16, xr,
+                          k0 * kQ4Block + (c & 15) * 16, p.cols, x_aligned);
+        };
 #pragma unroll
         for (int i = 0; i < kDepth - 1; ++i) {
             if (wk + i * warps_k < stages) load(wk + i * warps_k, i);
@@ -301,13 +306,22 @@ __global__ void __launch_bounds__(32 * kMmaWarps, 2) q4_mma_kernel(const MatvecP
                 if (next < stages) load(next, slot == 0 ? kDepth - 1 : slot - 1);
                 cp_async_commit();
             }
+            const uint8_t *a = ring + slot * stage_bytes + g * kStageARow + 4 * t;
+            const uint32_t turn = g * 16;
+            const uint8_t *x = ring + slot * stage_bytes + kStageA + kStageS + xg * kStageXRow + 4 * t;
+            /* the scales (and minima) of rows g and g + 8 */
+            using Pack = std::conditional_t<kGroups == 8, uint4, std::conditional_t<kGroups == 4, uint2, uint32_t>>;
+            const Pack *sc = (const Pack *)(ring + slot * stage_bytes + kStageA) + g;
+            union Row {
+                Pack all;
+                __half one[kGroups];
+                __device__ Row() {}
+            } scale[2], low[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) sm[h][i] = sm_next[h][i];
-            if (st + warps_k < stages) load_scales(st + warps_k, sm_next);
-            const uint32_t a = ring + slot * stage_bytes + g * (kStageBlocks * 16 + 16) + 4 * t;
-            const uint32_t x = ring + slot * stage_bytes + kStageA + xg * kStageXRow + 4 * t;
+            for (int h = 0; h < 2; ++h) {
+                scale[h].all = sc[8 * h];
+                if (kMin) low[h].all = sc[16 + 8 * h];
+            }
             const int left = nb - st * kStageBlocks; /* blocks from this stage on */
 #pragma unroll
             for (int gr = 0; gr < kGroups; ++gr) {
@@ -316,11 +330,9 @@ __global__ void __launch_bounds__(32 * kMmaWarps, 2) q4_mma_kernel(const MatvecP
 #pragma unroll
                 for (int k = gr * kPer; k < (gr + 1) * kPer; ++k) {
                     /* blocks behind the row's end hold zeros in the vectors */
-                    uint32_t w0, w1, x0, x1;
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0) : "r"(a + k * 16));
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1) : "r"(a + 8 * (kStageBlocks * 16 + 16) + k * 16));
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x0) : "r"(x + k * 32));
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x1) : "r"(x + k * 32 + 16));
+                    const uint32_t w0 = *(const uint32_t *)(a + (k * 16 ^ turn)),
+                                   w1 = *(const uint32_t *)(a + 8 * kStageARow + (k * 16 ^ turn));
+                    const uint32_t x0 = *(const uint32_t *)(x + k * 32), x1 = *(const uint32_t *)(x + k * 32 + 16);
                     const uint32_t av[4] = {((w0 << 4) & 0xf0f0f0f0u) ^ 0x80808080u, ((w1 << 4) & 0xf0f0f0f0u) ^ 0x80808080u,
                                             (w0 & 0xf0f0f0f0u) ^ 0x80808080u, (w1 & 0xf0f0f0f0u) ^ 0x80808080u};
                     mma_s8(c, av, x0, x1);
@@ -331,22 +343,21 @@ __global__ void __launch_bounds__(32 * kMmaWarps, 2) q4_mma_kernel(const MatvecP
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t both = __shfl_sync(0xffffffffu, sm[h][gr / 4], (lane & ~3) | (gr & 3));
-                    const float s = __half2float(__ushort_as_half((unsigned short)both));
+                    const float s = __half2float(scale[h].one[gr]);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        acc[2 * h + i] = fmaf(s * 0.0625f, (float)c[2 * h + i], acc[2 * h + i]);
+                    for (int i = 0; i < 2; ++i) acc[2 * h + i] = fmaf(s, (float)c[2 * h + i], acc[2 * h + i]);
                     if (kMin) {
-                        const float m = fmaf(8.0f, s, __half2float(__ushort_as_half((unsigned short)(both >> 16))));
+                        const float m = fmaf(8.0f, s, __half2float(low[h].one[gr]));
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            acc[2 * h + i] = fmaf(m * 0.0625f, (float)cx[i], acc[2 * h + i]);
+                        for (int i = 0; i < 2; ++i) acc[2 * h + i] = fmaf(m, (float)cx[i], acc[2 * h + i]);
                     }
                 }
             }
             slot = slot + 1 == kDepth ? 0 : slot + 1;
         }
         cp_async_wait<0>();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] *= 0.0625f;
     }
     if (warps_k == 1) {
         if (live)
@@ -357,7 +368,9 @@ __global__ void __launch_bounds__(32 * kMmaWarps, 2) q4_mma_kernel(const MatvecP
             }
         return;
     }
-    /* the warps of a row tile, in order */
+    /* the warps of a row tile, in order; their sums take the rings' place */
+    __syncthreads();
+    float(*part)[16 * kMmaStreams] = (float(*)[16 * kMmaStreams])smem;
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[warp][(2 * t + (i & 1)) * 16 + g + (i >> 1) * 8] = acc[i];
     __syncthreads();
@@ -379,7 +392,7 @@ cudaError_t launch_mma(const MatvecParams &p, int num_sms, cudaStream_t st) {
     const int tiles = (p.rows + 15) / 16, stages = (q4_blocks(p.cols) + kStageBlocks - 1) / kStageBlocks;
     int wk = 1;
     while (wk < kMmaWarps && 2 * wk <= stages && (long long)tiles * wk < 16LL * num_sms) wk *= 2;
-    const int smem = kMmaWarps * kDepth * (kStageA + std::min(kMmaStreams, p.streams) * kStageXRow);
+    const int smem = kMmaWarps * kDepth * (kStageA + kStageS + std::min(kMmaStreams, p.streams) * kStageXRow);
     const void *fn = (const void *)q4_mma_kernel<kGroup, kMin, kDepth>;
     cudaError_t e = raise_smem(fn, kMmaSmem);
     if (e != cudaSuccess) return e;
@@ -390,8 +403,7 @@ cudaError_t launch_mma(const MatvecParams &p, int num_sms, cudaStream_t st) {
 }
 
 template <int kGroup, bool kMin> cudaError_t launch_matvec(const MatvecParams &p, int num_sms, cudaStream_t st) {
-    /* two CTAs of at most 110 KB a SM */
-    return p.streams <= 4 ? launch_mma<kGroup, kMin, 4>(p, num_sms, st) : launch_mma<kGroup, kMin, 3>(p, num_sms, st);
+    return p.streams <= 3 ? launch_mma<kGroup, kMin, 4>(p, num_sms, st) : launch_mma<kGroup, kMin, 3>(p, num_sms, st);
 }
 
 template <int kGroup> cudaError_t launch_matvec(const MatvecParams &p, int num_sms, cudaStream_t st) {
