@@ -27,116 +27,201 @@ __host__ __device__ inline int q4_blocks(int cols) { return (cols + kQ4Block - 1
 
 /* ---------------------------------------------------------- quantizer --- */
 
-/* v >= 0 in f16, rounded up: with a scale that is not below max|w| / 7 no
- * weight is clamped.  Infinite when v is above f16's range. */
-__device__ __forceinline__ __half half_up(double v) {
-    const __half h = __double2half(v);
-    return (double)__half2float(h) < v ? __ushort_as_half(__half_as_ushort(h) + 1) : h;
-}
-/* v >= 0 in f16, rounded down */
-__device__ __forceinline__ __half half_down(double v) {
-    const __half h = __double2half(v);
-    return (double)__half2float(h) > v ? __ushort_as_half(__half_as_ushort(h) - 1) : h;
-}
-
 /* rint((w - m) / s) of the quotient in 64 bits: 32 bits where they cannot be
- * on the wrong side of a border (the quotient is below 16, its error below
- * 16 * 2 * 2^-24 < 2e-6) */
-__device__ __forceinline__ int q4_round(float w, float m, float s) {
-    const float t = __fdiv_rn(__fsub_rn(w, m), s);
-    const float n = rintf(t);
-    if (fabsf(t - n) < 0.5f - 4e-6f) return (int)n;
+ * on the wrong side of a border (the quotient is below 16, and three roundings
+ * of 2^-24 each are below 3e-6) */
+__device__ __noinline__ int q4_round64(float w, float m, float s) {
     return (int)rint(((double)w - (double)m) / (double)s);
 }
+__device__ __forceinline__ int q4_round(float w, float m, float s, float r) {
+    const float t = __fmul_rn(__fsub_rn(w, m), r);
+    const float n = rintf(t);
+    if (fabsf(t - n) < 0.5f - 4e-6f) return (int)n;
+    return q4_round64(w, m, s);
+}
 
-struct QuantParams {
-    const void *w;
-    long long w_stride;
-    int rows, cols, group;
-    uint8_t *q;
-    __half *scale, *min;
-};
-
-/* A warp takes a group: lane j the columns j, j + 32, ... */
-template <typename T, bool kMin>
-__global__ void __launch_bounds__(256) quantize_q4_kernel(const QuantParams p) {
-    const int lane = threadIdx.x & 31;
-    const int groups = (p.cols + p.group - 1) / p.group;
-    const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (at >= (long long)p.rows * groups) return;
-    const int row = (int)(at / groups), g = (int)(at - (long long)row * groups);
-    const T *w = (const T *)p.w + (size_t)row * p.w_stride;
-    const int c0 = g * p.group, c1 = min(p.cols, c0 + p.group);
-    float hi = -INFINITY, lo = INFINITY;
-    bool bad = false;
-    for (int c = c0 + lane; c < c1; c += 32) {
-        const float v = to_f32(w[c]);
-        bad |= !(fabsf(v) <= 3.4028234663852886e38f);
-        hi = fmaxf(hi, v);
-        lo = fminf(lo, v);
-    }
+/* Four elements from p on, of which n (may be below 0) exist. */
+template <typename T> __device__ __forceinline__ void get4(const T *p, int n, bool aligned, float (&v)[4]) {
+    if (n >= 4 && aligned) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 f = __ldg((const float4 *)p);
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        } else {
+            union Raw {
+                uint2 w;
+                T e[4];
+                __device__ Raw() {}
+            } raw;
+            raw.w = __ldg((const uint2 *)p);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    __half s, m = __float2half_rn(0.0f);
-    if (kMin) {
-        m = lo < 0.0f ? __hneg(half_up(-(double)lo)) : half_down((double)lo);
-        s = half_up(((double)hi - (double)__half2float(m)) / 15.0);
-        bad |= __hisinf(m) != 0;
-    } else {
-        s = half_up((double)fmaxf(hi, -lo) / 7.0);
-    }
-    bad |= __hisinf(s) != 0;
-    const float sf = __half2float(s), mf = __half2float(m);
-    for (int c = c0 + lane; c < c0 + p.group && c / kQ4Block < q4_blocks(p.cols); c += 32) {
-        int q = kMin ? 0 : 8;
-        if (c < c1 && !bad && sf > 0.0f) {
-            const int n = q4_round(to_f32(w[c]), kMin ? mf : 0.0f, sf);
-            q = kMin ? max(0, min(15, n)) : max(-7, min(7, n)) + 8;
+            for (int i = 0; i < 4; ++i) v[i] = to_f32(raw.e[i]);
         }
-        const int up = __shfl_down_sync(0xffffffffu, q, 16);
-        if (lane < 16)
-            p.q[(size_t)row * q4_blocks(p.cols) * 16 + c / kQ4Block * 16 + lane] = (uint8_t)(q | up << 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
     }
-    if (lane == 0) {
-        const __half nan = __ushort_as_half(0x7e00);
-        p.scale[(size_t)row * groups + g] = bad ? nan : s;
-        if (kMin) p.min[(size_t)row * groups + g] = bad ? nan : m;
+}
+template <typename T> __device__ __forceinline__ void put4(T *p, int n, bool aligned, const float (&v)[4]) {
+    if (n >= 4 && aligned) {
+        if constexpr (sizeof(T) == 4) {
+            *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            union Raw {
+                uint2 w;
+                T e[4];
+                __device__ Raw() {}
+            } raw;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw.e[i] = from_f32<T>(v[i]);
+            *(uint2 *)p = raw.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) p[i] = from_f32<T>(v[i]);
     }
 }
 
-/* ---------------------------------------------------------- read-back --- */
-struct BackParams {
-    const uint8_t *q;
-    const __half *scale, *min;
+/* Both directions: a lane takes a 32-bit word, columns 4u .. 4u + 3 and 16 +
+ * 4u .. of a block; a warp takes kRun runs of 256 columns of a row, all their
+ * loads at once. */
+constexpr int kRun = 4;
+constexpr int kQ4Warps = 8;
+struct ConvertParams {
+    uint8_t *q;
+    __half *scale, *min;
     int rows, cols, group;
     void *w;
     long long w_stride;
+    int aligned; /* rows of w are aligned to four elements */
 };
+inline long long q4_runs(int rows, int cols) { return (long long)rows * ((cols + 255) / 256); }
+inline unsigned q4_ctas(int rows, int cols) {
+    return (unsigned)((q4_runs(rows, cols) + kRun * kQ4Warps - 1) / (kRun * kQ4Warps));
+}
 
-/* A thread takes four consecutive columns. */
-template <typename T, bool kMin>
-__global__ void __launch_bounds__(256) dequantize_q4_kernel(const BackParams p) {
-    const int quads = (p.cols + 3) / 4;
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (long long)p.rows * quads) return;
-    const int row = (int)(at / quads), c = (int)(at - (long long)row * quads) * 4;
-    const int groups = (p.cols + p.group - 1) / p.group;
-    const size_t block = (size_t)row * q4_blocks(p.cols) + c / kQ4Block;
-    const uint32_t word = __ldg((const uint32_t *)(p.q + block * 16) + (c % 16) / 4);
-    const uint32_t four = (c % kQ4Block >= 16 ? word >> 4 : word) & 0x0f0f0f0fu;
-    const float s = __half2float(p.scale[(size_t)row * groups + c / p.group]);
-    const float m = kMin ? __half2float(p.min[(size_t)row * groups + c / p.group]) : 0.0f;
-    T *w = (T *)p.w + (size_t)row * p.w_stride + c;
+template <typename T, int kGroup, bool kMin>
+__global__ void __launch_bounds__(32 * kQ4Warps) quantize_q4_kernel(const ConvertParams p) {
+    const int lane = threadIdx.x & 31, nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
+    const int per_row = (p.cols + 255) / 256;
+    const long long run0 = ((long long)blockIdx.x * kQ4Warps + (threadIdx.x >> 5)) * kRun;
+    float v[kRun][8];
+    int row = (int)(run0 / per_row), seg = (int)(run0 - (long long)row * per_row);
+    const int row_0 = row, seg_0 = seg;
+    auto step = [&] {
+        if (++seg == per_row) seg = 0, ++row;
+    };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float q = (float)((four >> (8 * j)) & 15u);
-        /* s * q is exact in 32 bits (11 and 4 bits): one rounding */
-        const float v = kMin ? fmaf(s, q, m) : __fmul_rn(s, q - 8.0f);
-        if (c + j < p.cols) w[j] = from_f32<T>(v);
+    for (int u = 0; u < kRun; ++u, step()) {
+        if (row >= p.rows) break;
+        const int c = seg * 256 + (lane >> 2) * 32 + (lane & 3) * 4;
+        const T *w = (const T *)p.w + (size_t)row * p.w_stride + c;
+        float lo[4], hi[4];
+        get4(w, p.cols - c, p.aligned, lo);
+        get4(w + 16, p.cols - c - 16, p.aligned, hi);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[u][i] = lo[i], v[u][4 + i] = hi[i];
+    }
+    row = row_0, seg = seg_0;
+#pragma unroll
+    for (int u = 0; u < kRun; ++u, step()) {
+        if (row >= p.rows) break;
+        const int c = seg * 256 + (lane >> 2) * 32 + (lane & 3) * 4;
+        /* what does not exist is 0 to the absolute largest, and left out of the extremes */
+        float hi = -INFINITY, lo = INFINITY, top = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool in = c + (i < 4 ? i : 12 + i) < p.cols;
+            const float a = fabsf(v[u][i]);
+            bad |= !(a <= 3.4028234663852886e38f);
+            top = fmaxf(top, a);
+            if (kMin && in) hi = fmaxf(hi, v[u][i]), lo = fminf(lo, v[u][i]);
+        }
+        int worst = bad ? 0x7f800000 : __float_as_int(top);
+#pragma unroll
+        for (int o = kGroup / 16; o > 0; o >>= 1) { /* 4 lanes a block */
+            worst = max(worst, __shfl_xor_sync(0xffffffffu, worst, o));
+            if (kMin) {
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            }
+        }
+        bad = worst >= 0x7f800000;
+        /* Rounded outwards step by step, which is rounding outwards once: f16
+         * numbers and their multiples by 7 or 15 are fp32 numbers too. */
+        __half s, m = __float2half_rn(0.0f);
+        if (kMin) {
+            m = __float2half_rd(lo);
+            s = __float2half_ru(__fdiv_ru(__fsub_ru(hi, __half2float(m)), 15.0f));
+            bad |= __hisinf(m) != 0;
+        } else {
+            s = __float2half_ru(__fdiv_ru(__int_as_float(worst), 7.0f));
+        }
+        bad |= __hisinf(s) != 0;
+        const float sf = __half2float(s), mf = __half2float(m);
+        const bool some = !bad && sf > 0.0f;
+        const float r = some ? __frcp_rn(sf) : 0.0f;
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            int q = kMin ? 0 : 8;
+            if (some) {
+                const int n = q4_round(v[u][i], mf, sf, r);
+                q = kMin ? max(0, min(15, n)) : max(-7, min(7, n)) + 8;
+            }
+            word |= (uint32_t)q << (i < 4 ? 8 * i : 8 * (i - 4) + 4);
+        }
+        if (c / kQ4Block < nb) {
+            ((uint32_t *)p.q)[((size_t)row * nb + c / kQ4Block) * 4 + (lane & 3)] = word;
+            if (c % kGroup == 0) {
+                const __half nan = __ushort_as_half(0x7e00);
+                p.scale[(size_t)row * groups + c / kGroup] = bad ? nan : s;
+                if (kMin) p.min[(size_t)row * groups + c / kGroup] = bad ? nan : m;
+            }
+        }
+    }
+}
+
+template <typename T, int kGroup, bool kMin>
+__global__ void __launch_bounds__(32 * kQ4Warps) dequantize_q4_kernel(const ConvertParams p) {
+    const int lane = threadIdx.x & 31, nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
+    const int per_row = (p.cols + 255) / 256;
+    const long long run0 = ((long long)blockIdx.x * kQ4Warps + (threadIdx.x >> 5)) * kRun;
+    int row = (int)(run0 / per_row), seg = (int)(run0 - (long long)row * per_row);
+    const int row_0 = row, seg_0 = seg;
+    auto step = [&] {
+        if (++seg == per_row) seg = 0, ++row;
+    };
+    uint32_t word[kRun];
+    float s[kRun], m[kRun];
+#pragma unroll
+    for (int u = 0; u < kRun; ++u, step()) {
+        const int c = seg * 256 + (lane >> 2) * 32;
+        if (row >= p.rows) break;
+        if (c >= p.cols) continue;
+        word[u] = __ldg((const uint32_t *)p.q + ((size_t)row * nb + c / kQ4Block) * 4 + (lane & 3));
+        s[u] = __half2float(p.scale[(size_t)row * groups + c / kGroup]);
+        m[u] = kMin ? __half2float(p.min[(size_t)row * groups + c / kGroup]) : 0.0f;
+    }
+    row = row_0, seg = seg_0;
+#pragma unroll
+    for (int u = 0; u < kRun; ++u, step()) {
+        const int c = seg * 256 + (lane >> 2) * 32 + (lane & 3) * 4;
+        if (row >= p.rows) break;
+        if (c >= p.cols) continue;
+        T *w = (T *)p.w + (size_t)row * p.w_stride + c;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float q = (float)((word[u] >> (8 * i + 4 * h)) & 15u);
+                /* s * q is exact in 32 bits (11 and 4 bits): one rounding */
+                v[i] = kMin ? fmaf(s[u], q, m[u]) : __fmul_rn(s[u], q - 8.0f);
+            }
+            put4(w + 16 * h, p.cols - c - 16 * h, p.aligned, v);
+        }
     }
 }
 
@@ -234,6 +319,158 @@ __device__ __forceinline__ void store_y(const MatvecParams &p, int b, int row, f
         ((__nv_bfloat16 *)p.y)[at] = __float2bfloat16_rn(v);
     else
         ((__half *)p.y)[at] = __float2half_rn(v);
+}
+
+/* ---- one or two streams: 4-way int8 dot products ----
+ *
+ * A warp takes kR rows; a lane takes every 32nd block of each (16 bytes, all
+ * kR loads at once), eight dp4a a block and stream, and one scaled addition
+ * in fp32.  The vectors lie in shared memory as two planes, columns 0-15 and
+ * 16-31 of the blocks, so that a warp's 16-byte reads have no bank conflicts.
+ * With few rows the K range of a row is split over warps of the CTA. */
+constexpr int kDotWarps = 8;
+
+template <int kB, int kR, bool kMin>
+__global__ void __launch_bounds__(32 * kDotWarps) q4_dot_kernel(const MatvecParams p, int warps_k, int group_shift) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int nb = q4_blocks(p.cols), groups = ((nb - 1) >> group_shift) + 1;
+    uint4 *xs = (uint4 *)smem; /* [kB][2][nb] */
+    int *sums = (int *)(smem + (size_t)kB * nb * 32); /* [kB][nb] */
+    const bool x_aligned = (((uintptr_t)p.x | (uintptr_t)p.x_stride) & 15) == 0;
+    for (int c = threadIdx.x; c < kB * nb * 2; c += 32 * kDotWarps) {
+        const int b = kB == 1 ? 0 : c / (nb * 2), i = c - b * nb * 2;
+        stage_x16((uint8_t *)(xs + (size_t)(b * 2 + (i & 1)) * nb + (i >> 1)), p.x + b * p.x_stride, i * 16, p.cols,
+                  x_aligned);
+    }
+    const int wk = warp % warps_k;
+    const int row0 = (blockIdx.x * (kDotWarps / warps_k) + warp / warps_k) * kR;
+    const uint4 *q[kR];
+    const __half *s[kR], *m[kR];
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+        const int row = min(row0 + r, p.rows - 1);
+        q[r] = (const uint4 *)p.q + (size_t)row * nb;
+        s[r] = p.scale + (size_t)row * groups;
+        m[r] = p.min + (size_t)row * groups;
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
+    if (kMin) {
+        for (int c = threadIdx.x; c < kB * nb; c += 32 * kDotWarps) {
+            const int b = kB == 1 ? 0 : c / nb, i = c - b * nb;
+            const uint4 lo = xs[(size_t)(b * 2) * nb + i], hi = xs[(size_t)(b * 2 + 1) * nb + i];
+            int sum = 0;
+            for (uint32_t v : {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}) sum = __dp4a((int)v, 0x10101010, sum);
+            sums[c] = sum; /* 16 times the sum, as the dots */
+        }
+        __syncthreads();
+    }
+    float acc[kR][kB] = {};
+    constexpr int kU = kR >= 4 ? 1 : 4 / kR; /* blocks of a row in flight */
+    if (row0 < p.rows) {
+        for (int k0 = wk * 32 + lane; k0 < nb; k0 += 32 * kU * warps_k) {
+            uint4 v[kU][kR];
+            float sc[kU][kR], lo[kU][kR];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int k = k0 + 32 * u * warps_k;
+#pragma unroll
+                for (int r = 0; r < kR; ++r) {
+                    if (k >= nb) break;
+                    v[u][r] = __ldg(q[r] + k);
+                    sc[u][r] = __half2float(__ldg(s[r] + (k >> group_shift)));
+                    if (kMin) lo[u][r] = __half2float(__ldg(m[r] + (k >> group_shift)));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int k = k0 + 32 * u * warps_k;
+                if (k >= nb) break;
+#pragma unroll
+                for (int b = 0; b < kB; ++b) {
+                    const uint4 xl = xs[(size_t)(b * 2) * nb + k], xh = xs[(size_t)(b * 2 + 1) * nb + k];
+                    const uint32_t x0[4] = {xl.x, xl.y, xl.z, xl.w}, x1[4] = {xh.x, xh.y, xh.z, xh.w};
+                    const float sum = kMin ? (float)sums[b * nb + k] : 0.0f;
+#pragma unroll
+                    for (int r = 0; r < kR; ++r) {
+                        const uint32_t w[4] = {v[u][r].x, v[u][r].y, v[u][r].z, v[u][r].w};
+                        int dot = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            dot = __dp4a((int)(((w[i] << 4) & 0xf0f0f0f0u) ^ 0x80808080u), (int)x0[i], dot);
+                            dot = __dp4a((int)((w[i] & 0xf0f0f0f0u) ^ 0x80808080u), (int)x1[i], dot);
+                        }
+                        acc[r][b] = fmaf(sc[u][r], (float)dot, acc[r][b]);
+                        if (kMin) acc[r][b] = fmaf(fmaf(8.0f, sc[u][r], lo[u][r]), sum, acc[r][b]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kR; ++r)
+#pragma unroll
+        for (int b = 0; b < kB; ++b) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) acc[r][b] += __shfl_xor_sync(0xffffffffu, acc[r][b], o);
+            acc[r][b] *= 0.0625f;
+        }
+    if (warps_k == 1) {
+        if (lane == 0)
+#pragma unroll
+            for (int r = 0; r < kR; ++r)
+#pragma unroll
+                for (int b = 0; b < kB; ++b)
+                    if (row0 + r < p.rows) store_y(p, b, row0 + r, acc[r][b]);
+        return;
+    }
+    /* the warps of a row, in order */
+    __shared__ float part[kDotWarps][kR * kB];
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < kR * kB; ++i) part[warp][i] = acc[i / kB][i % kB];
+    __syncthreads();
+    const int tiles = kDotWarps / warps_k;
+    for (int i = threadIdx.x; i < tiles * kR * kB; i += 32 * kDotWarps) {
+        const int tile = i / (kR * kB), j = i % (kR * kB);
+        const int row = (blockIdx.x * tiles + tile) * kR + j / kB;
+        float sum = 0.0f;
+        for (int w = 0; w < warps_k; ++w) sum += part[tile * warps_k + w][j];
+        if (row < p.rows) store_y(p, j % kB, row, sum);
+    }
+}
+
+constexpr int kDotSmem = 96 * 1024;
+
+inline int dot_smem(const MatvecParams &p, int streams) {
+    const long long n = (long long)streams * q4_blocks(p.cols) * (32 + (p.min ? 4 : 0));
+    return n > kDotSmem ? -1 : (int)n;
+}
+
+template <int kB, int kR, bool kMin> cudaError_t launch_dot(const MatvecParams &p, int num_sms, cudaStream_t st) {
+    const int nb = q4_blocks(p.cols), tiles = (p.rows + kR - 1) / kR;
+    int wk = 1;
+    while (wk < kDotWarps && 32 * wk < nb && (long long)tiles * wk < 16LL * num_sms) wk *= 2;
+    const void *fn = (const void *)q4_dot_kernel<kB, kR, kMin>;
+    cudaError_t e = raise_smem(fn, kDotSmem);
+    if (e != cudaSuccess) return e;
+    const int per = kDotWarps / wk, shift = p.group == 32 ? 0 : p.group == 64 ? 1 : 2;
+    q4_dot_kernel<kB, kR, kMin><<<(tiles + per - 1) / per, 32 * kDotWarps, dot_smem(p, kB), st>>>(p, wk, shift);
+    return cudaGetLastError();
+}
+
+template <int kB> cudaError_t launch_dot(const MatvecParams &p, int num_sms, cudaStream_t st) {
+    /* rows a warp: four once that leaves 24 warps an SM */
+    const int per_warp = p.rows / (24 * num_sms);
+    if (p.min)
+        return per_warp >= 4   ? launch_dot<kB, 4, true>(p, num_sms, st)
+               : per_warp >= 2 ? launch_dot<kB, 2, true>(p, num_sms, st)
+                               : launch_dot<kB, 1, true>(p, num_sms, st);
+    return per_warp >= 4   ? launch_dot<kB, 4, false>(p, num_sms, st)
+           : per_warp >= 2 ? launch_dot<kB, 2, false>(p, num_sms, st)
+                           : launch_dot<kB, 1, false>(p, num_sms, st);
 }
 
 template <int kGroup, bool kMin, int kDepth>
@@ -410,13 +647,20 @@ template <int kGroup> cudaError_t launch_matvec(const MatvecParams &p, int num_s
     return p.min != nullptr ? launch_matvec<kGroup, true>(p, num_sms, st) : launch_matvec<kGroup, false>(p, num_sms, st);
 }
 
-/* calls f with the type of `dtype` and the truth of `min` as constants */
-template <typename F> cudaError_t by_type(int dtype, bool min, F f) {
-    if (dtype == LAL_TAIL_F32)
-        return min ? f(float{}, std::true_type{}) : f(float{}, std::false_type{});
-    if (dtype == LAL_TAIL_BF16)
-        return min ? f(__nv_bfloat16{}, std::true_type{}) : f(__nv_bfloat16{}, std::false_type{});
-    return min ? f(__half{}, std::true_type{}) : f(__half{}, std::false_type{});
+/* one of the conversions' kernels by type, group and minimum */
+template <typename T, int kGroup>
+cudaError_t launch_convert(const ConvertParams &p, bool back, cudaStream_t st) {
+    const unsigned n = q4_ctas(p.rows, p.cols);
+    if (back && p.min) dequantize_q4_kernel<T, kGroup, true><<<n, 32 * kQ4Warps, 0, st>>>(p);
+    else if (back) dequantize_q4_kernel<T, kGroup, false><<<n, 32 * kQ4Warps, 0, st>>>(p);
+    else if (p.min) quantize_q4_kernel<T, kGroup, true><<<n, 32 * kQ4Warps, 0, st>>>(p);
+    else quantize_q4_kernel<T, kGroup, false><<<n, 32 * kQ4Warps, 0, st>>>(p);
+    return cudaGetLastError();
+}
+template <typename T> cudaError_t launch_convert(const ConvertParams &p, bool back, cudaStream_t st) {
+    return p.group == 32   ? launch_convert<T, 32>(p, back, st)
+           : p.group == 64 ? launch_convert<T, 64>(p, back, st)
+                           : launch_convert<T, 128>(p, back, st);
 }
 
 int check_weights(const char *op, const lal_tail_q4 *w) {
@@ -446,12 +690,7 @@ struct WeightSpans {
     bool meet_each_other() const { return q.meets(s) || q.meets(m) || s.meets(m); }
 };
 
-}  // namespace
-
-extern "C" {
-
-int lal_tail_quantize_q4(const lal_tail_q4 *w, const void *d_w, int64_t w_stride, int dtype, void *stream) {
-    static const char *op = "quantize_q4";
+int convert_q4(const char *op, const lal_tail_q4 *w, void *d_w, int64_t w_stride, int dtype, bool back, void *stream) {
     if (const int rc = check_weights(op, w)) return rc;
     const int size = dtype_size(dtype);
     if (size == 0) return layer_fail(LAL_TAIL_ERR_ARG, "%s: dtype %d", op, dtype);
@@ -462,49 +701,31 @@ int lal_tail_quantize_q4(const lal_tail_q4 *w, const void *d_w, int64_t w_stride
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: a pointer is not aligned to its type", op);
     const WeightSpans spans(w);
     if (spans.meets(Span(d_w, w->rows, w->cols, w_stride, size)) || spans.meet_each_other())
-        return layer_fail(LAL_TAIL_ERR_ARG, "%s: an output overlaps another buffer", op);
+        return layer_fail(LAL_TAIL_ERR_ARG, "%s: buffers overlap", op);
+    if (q4_runs(w->rows, w->cols) / (kRun * kQ4Warps) >= 0x7fffffffLL)
+        return layer_fail(LAL_TAIL_ERR_UNSUPPORTED, "%s: weights of %d x %d", op, w->rows, w->cols);
     static const char *const names[] = {"d_w", "d_q", "d_scale", "d_min"};
     const void *ptrs[] = {d_w, w->d_q, w->d_scale, w->d_min};
     CallDevice dev;
     if (const int rc = dev.enter(op, names, ptrs, 4)) return rc;
-    const QuantParams p = {d_w, w_stride, w->rows, w->cols, w->group, w->d_q, (__half *)w->d_scale,
-                           (__half *)w->d_min};
-    const long long warps = (long long)w->rows * ((w->cols + w->group - 1LL) / w->group);
-    if ((warps + 7) / 8 > 0x7fffffffLL)
-        return layer_fail(LAL_TAIL_ERR_UNSUPPORTED, "%s: weights of %d x %d", op, w->rows, w->cols);
-    return launched(op, by_type(dtype, w->d_min != nullptr, [&](auto t, auto min) {
-        quantize_q4_kernel<decltype(t), decltype(min)::value>
-            <<<(unsigned)((warps + 7) / 8), 256, 0, (cudaStream_t)stream>>>(p);
-        return cudaGetLastError();
-    }));
+    const ConvertParams p = {w->d_q, (__half *)w->d_scale, (__half *)w->d_min, w->rows, w->cols, w->group, d_w, w_stride,
+                             ((uintptr_t)d_w | (uintptr_t)w_stride * size) % (4 * size) == 0};
+    cudaStream_t st = (cudaStream_t)stream;
+    return launched(op, dtype == LAL_TAIL_F32    ? launch_convert<float>(p, back, st)
+                        : dtype == LAL_TAIL_BF16 ? launch_convert<__nv_bfloat16>(p, back, st)
+                                                 : launch_convert<__half>(p, back, st));
+}
+
+}  // namespace
+
+extern "C" {
+
+int lal_tail_quantize_q4(const lal_tail_q4 *w, const void *d_w, int64_t w_stride, int dtype, void *stream) {
+    return convert_q4("quantize_q4", w, (void *)d_w, w_stride, dtype, false, stream);
 }
 
 int lal_tail_dequantize_q4(const lal_tail_q4 *w, void *d_w, int64_t w_stride, int dtype, void *stream) {
-    static const char *op = "dequantize_q4";
-    if (const int rc = check_weights(op, w)) return rc;
-    const int size = dtype_size(dtype);
-    if (size == 0) return layer_fail(LAL_TAIL_ERR_ARG, "%s: dtype %d", op, dtype);
-    if (w->rows == 0) return LAL_TAIL_OK;
-    if (!d_w) return layer_fail(LAL_TAIL_ERR_ARG, "%s: a null pointer", op);
-    if (w_stride < w->cols) return layer_fail(LAL_TAIL_ERR_ARG, "%s: a stride below cols %d", op, w->cols);
-    if ((uintptr_t)d_w % size != 0)
-        return layer_fail(LAL_TAIL_ERR_ARG, "%s: a pointer is not aligned to its type", op);
-    if (WeightSpans(w).meets(Span(d_w, w->rows, w->cols, w_stride, size)))
-        return layer_fail(LAL_TAIL_ERR_ARG, "%s: an output overlaps another buffer", op);
-    static const char *const names[] = {"d_w", "d_q", "d_scale", "d_min"};
-    const void *ptrs[] = {d_w, w->d_q, w->d_scale, w->d_min};
-    CallDevice dev;
-    if (const int rc = dev.enter(op, names, ptrs, 4)) return rc;
-    const BackParams p = {w->d_q, (const __half *)w->d_scale, (const __half *)w->d_min, w->rows, w->cols,
-                          w->group, d_w, w_stride};
-    const long long threads = (long long)w->rows * ((w->cols + 3LL) / 4);
-    if ((threads + 255) / 256 > 0x7fffffffLL)
-        return layer_fail(LAL_TAIL_ERR_UNSUPPORTED, "%s: weights of %d x %d", op, w->rows, w->cols);
-    return launched(op, by_type(dtype, w->d_min != nullptr, [&](auto t, auto min) {
-        dequantize_q4_kernel<decltype(t), decltype(min)::value>
-            <<<(unsigned)((threads + 255) / 256), 256, 0, (cudaStream_t)stream>>>(p);
-        return cudaGetLastError();
-    }));
+    return convert_q4("dequantize_q4", w, d_w, w_stride, dtype, true, stream);
 }
 
 int lal_tail_q4_matvec(const lal_tail_q4 *w, const int8_t *d_xq, int64_t xq_stride, const float *d_scale_x,
@@ -534,6 +755,7 @@ int lal_tail_q4_matvec(const lal_tail_q4 *w, const int8_t *d_xq, int64_t xq_stri
                             (const __half *)w->d_min, n_streams, w->rows, w->cols, w->group, d_y, y_stride, dtype};
     cudaStream_t st = (cudaStream_t)stream;
     const int sms = dev.num_sms();
+    if (n_streams == 1 && dot_smem(p, n_streams) >= 0) return launched(op, launch_dot<1>(p, sms, st));
     return launched(op, w->group == 32   ? launch_matvec<32>(p, sms, st)
                         : w->group == 64 ? launch_matvec<64>(p, sms, st)
                                          : launch_matvec<128>(p, sms, st));

@@ -2,9 +2,9 @@
  * tail_q8.cu -- rows quantized to 8 bits as they are computed: what feeds the
  * 4-bit products of a layer (tail_q4.cu).
  *
- *   norm_q8_kernel    h = x + residual (rounded to its type), v = h * w,
- *                     scale = max|v| / sqrt(mean h^2 + eps) / 127
- *   swiglu_q8_kernel  v = gate / (1 + exp(-gate)) * up, scale = max|v| / 127
+ *   NormRow    h = x + residual (rounded to its type), v = h * w,
+ *              scale = max|v| / sqrt(mean h^2 + eps) / 127
+ *   SwigluRow  v = gate / (1 + exp(-gate)) * up, scale = max|v| / 127
  *
  * and q = rint(127 v / max|v|), ties to even, as in 64 bits: the norm's factor
  * cancels in q, so one reduction gives both the sum of squares and max|v|.
@@ -19,140 +19,11 @@
 #include "tail_layer.h"
 
 #include <cmath>
+#include <cstring>
 
 using namespace lal;
 
 namespace {
-
-constexpr int kRowThreads = 256;
-constexpr float kFltMax = 3.4028234663852886e38f;
-/* |v| in 32 bits at or above kWideHi or (not zero) below kWideLo: the row is
- * computed in 64 bits, clear of overflow and of denormal rounding */
-constexpr float kWideHi = 1e37f, kWideLo = 1e-30f;
-
-/* One element of a row, in 32 and in 64 bits. */
-template <typename T> struct NormRow {
-    const T *x, *r;
-    T *h;
-    const float *w;
-    /* |error of v()| <= 2^-24, of 127/max|v| 2^-24, of their product 2^-24: 3 * 2^-24 * 127 < 3e-5 */
-    static constexpr float kBorder = 3e-5f;
-    static constexpr bool kNorm = true;
-    struct Elem {
-        float h, w;
-        __device__ float v() const { return __fmul_rn(h, w); }
-        __device__ double v64() const { return (double)h * (double)w; }
-        __device__ bool zero() const { return h == 0.0f || w == 0.0f; }
-    };
-    /* first visit: adds the residual and stores the sum */
-    __device__ Elem first(int i) const {
-        float a = to_f32(x[i]);
-        if (r != nullptr) a = to_f32(from_f32<T>(__fadd_rn(a, to_f32(r[i]))));
-        if (h != nullptr) h[i] = from_f32<T>(a);
-        return {a, __ldg(w + i)};
-    }
-    /* second visit, by the thread that made the first */
-    __device__ Elem again(int i) const { return {to_f32(h != nullptr ? h[i] : x[i]), __ldg(w + i)}; }
-};
-
-template <typename T> struct SwigluRow {
-    const T *g, *u;
-    /* expf 2 ulp, 1 + e, the division and the product 0.5 ulp each (2^-23), then as above:
-     * (3.5 * 2^-23 + 2 * 2^-24) * 127 < 7e-5 */
-    static constexpr float kBorder = 1e-4f;
-    static constexpr bool kNorm = false;
-    struct Elem {
-        float g, u;
-        __device__ float v() const { return __fmul_rn(__fdiv_rn(g, 1.0f + expf(-g)), u); }
-        __device__ double v64() const { return (double)g / (1.0 + exp(-(double)g)) * (double)u; }
-        __device__ bool zero() const { return g == 0.0f || u == 0.0f; }
-    };
-    __device__ Elem first(int i) const { return {to_f32(g[i]), to_f32(u[i])}; }
-    __device__ Elem again(int i) const { return first(i); }
-};
-
-/* A thread's part of a row's statistics. */
-struct RowStat {
-    double sum = 0.0;   /* of h^2 */
-    double top = 0.0;   /* max|v| in 64 bits; NaN or infinite if a v is */
-    float top32 = 0.0f;
-    bool wide = false;
-
-    template <typename E> __device__ void take(const E &e) {
-        const float a = fabsf(e.v());
-        if (!(a < kWideHi)) { /* NaN and infinities too */
-            wide = true;
-            const double d = fabs(e.v64());
-            if (!(d <= top)) top = top != top ? top : d;
-        } else if (a >= top32 * (1.0f - 1e-5f)) {
-            /* may be the largest: 64 bits decide (|error of v()| < 1e-6) */
-            if (a >= kWideLo || (top32 < 1e-25f && !e.zero())) {
-                const double d = fabs(e.v64());
-                if (d > top) top = d;
-            }
-            top32 = fmaxf(top32, a);
-        } else if (a < kWideLo && top32 < 1e-25f && !e.zero()) {
-            const double d = fabs(e.v64());
-            if (d > top) top = d;
-        }
-    }
-};
-
-__device__ __forceinline__ double max_or_nan(double a, double b) { return a != a || a > b ? a : b; }
-
-/* The row's statistics, in every thread. */
-__device__ __forceinline__ void block_stat(RowStat &s) {
-    __shared__ double sums[kRowThreads / 32], tops[kRowThreads / 32];
-    __shared__ int wides[kRowThreads / 32];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        s.sum += __shfl_xor_sync(0xffffffffu, s.sum, o);
-        s.top = max_or_nan(s.top, __shfl_xor_sync(0xffffffffu, s.top, o));
-    }
-    const bool wide = __any_sync(0xffffffffu, s.wide);
-    if ((threadIdx.x & 31) == 0) {
-        sums[threadIdx.x >> 5] = s.sum;
-        tops[threadIdx.x >> 5] = s.top;
-        wides[threadIdx.x >> 5] = wide;
-    }
-    __syncthreads();
-    s.sum = 0.0;
-    s.top = 0.0;
-    s.wide = false;
-#pragma unroll
-    for (int i = 0; i < kRowThreads / 32; ++i) {
-        s.sum += sums[i];
-        s.top = max_or_nan(s.top, tops[i]);
-        s.wide |= wides[i] != 0;
-    }
-    if (s.top < (double)kWideLo) s.wide = true;
-}
-
-/* A row's quantizer, once its statistics are known. */
-struct RowQuant {
-    double top;
-    float r32;     /* 127 / top */
-    float scale;
-    bool wide, empty; /* empty: every q is 0 */
-
-    /* factor: what v is still to be multiplied by (the norm's) */
-    __device__ RowQuant(const RowStat &s, double factor) : top(s.top), wide(s.wide) {
-        const double size = s.top == 0.0 ? 0.0 : s.top * factor; /* no eps: 0, not 0 * infinity */
-        const bool fine = size <= (double)kFltMax; /* false for NaN */
-        empty = !fine || s.top == 0.0;
-        scale = fine ? (float)(size / 127.0) : __int_as_float(0x7fc00000);
-        r32 = empty ? 0.0f : (float)(127.0 / s.top);
-    }
-    template <typename E> __device__ int q(const E &e, float border) const {
-        if (empty) return 0;
-        if (!wide) {
-            const float t = __fmul_rn(e.v(), r32);
-            const float n = rintf(t);
-            if (fabsf(t - n) < 0.5f - border) return (int)n;
-        }
-        return (int)rint(127.0 * e.v64() / top);
-    }
-};
 
 struct RowParams {
     const void *a, *b; /* x and the residual, or gate and up */
@@ -165,43 +36,352 @@ struct RowParams {
     float *scale;
 };
 
-template <typename Row> __device__ __forceinline__ void row_q8(const Row &row, const RowParams &p) {
-    RowStat s;
-    for (int i = threadIdx.x; i < p.n; i += kRowThreads) {
-        const auto e = row.first(i);
-        if constexpr (Row::kNorm) s.sum += (double)e.h * (double)e.h;
-        s.take(e);
+/* What few elements need, out of line: inlined for each of a thread's elements
+ * it would fill the instruction cache. */
+__device__ __noinline__ double silu64(double g, double u) { return g / (1.0 + exp(-g)) * u; }
+__device__ __noinline__ int round64(double v, double top) { return (int)rint(127.0 * v / top); }
+
+constexpr float kFltMax = 3.4028234663852886e38f;
+/* max|v| in 32 bits at or above kWideHi or (not zero) below kWideLo: the row
+ * is computed in 64 bits, clear of overflow and of denormal rounding */
+constexpr float kWideHi = 1e37f, kWideLo = 1e-30f;
+
+/* Eight elements of a row from p on, of which `n` exist, as wide as p's
+ * alignment allows (rows of 16-bit elements may begin at any even address). */
+template <typename T> __device__ __forceinline__ void get8(const T *p, int n, float (&v)[8]) {
+    if (n < 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
+        return;
     }
-    block_stat(s);
-    const RowQuant rq(s, Row::kNorm ? 1.0 / sqrt(s.sum / p.n + (double)p.eps) : 1.0);
-    int8_t *q = p.q + (size_t)blockIdx.x * p.q_stride;
-    for (int i = threadIdx.x; i < p.n; i += kRowThreads) q[i] = (int8_t)rq.q(row.again(i), Row::kBorder);
-    if (threadIdx.x == 0) p.scale[blockIdx.x] = rq.scale;
+    const unsigned at = (unsigned)(uintptr_t)p;
+    union Raw {
+        uint4 q[sizeof(T) / 2];
+        uint32_t w[2 * sizeof(T)];
+        T e[8];
+        __device__ Raw() {}
+    } raw;
+    if ((at & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw.q[i] = ((const uint4 *)p)[i];
+    } else if (sizeof(T) == 4 || (at & 3) == 0) {
+#pragma unroll
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) raw.w[i] = ((const uint32_t *)p)[i];
+    } else {
+        raw.e[0] = p[0];
+        const uint32_t *w = (const uint32_t *)(p + 1);
+        const uint32_t m0 = w[0], m1 = w[1], m2 = w[2];
+        const unsigned short last = ((const unsigned short *)p)[7];
+        const uint32_t first = *(const unsigned short *)&raw.e[0];
+        raw.w[0] = first | m0 << 16;
+        raw.w[1] = __funnelshift_r(m0, m1, 16);
+        raw.w[2] = __funnelshift_r(m1, m2, 16);
+        raw.w[3] = m2 >> 16 | (uint32_t)last << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(raw.e[i]);
 }
 
-/* One CTA a row, two visits to each element. */
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) norm_q8_kernel(const RowParams p) {
-    const size_t i = blockIdx.x;
-    const NormRow<T> row = {(const T *)p.a + i * p.a_stride,
-                            p.b != nullptr ? (const T *)p.b + i * p.b_stride : nullptr,
-                            p.h != nullptr ? (T *)p.h + i * p.h_stride : nullptr, p.w};
-    row_q8(row, p);
+template <typename T> __device__ __forceinline__ void put8(T *p, int n, const float (&v)[8]) {
+    if (n < 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = from_f32<T>(v[i]);
+        return;
+    }
+    const unsigned at = (unsigned)(uintptr_t)p;
+    union Raw {
+        uint4 q[sizeof(T) / 2];
+        uint32_t w[2 * sizeof(T)];
+        T e[8];
+        __device__ Raw() {}
+    } raw;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw.e[i] = from_f32<T>(v[i]);
+    if ((at & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((uint4 *)p)[i] = raw.q[i];
+    } else if (sizeof(T) == 4 || (at & 3) == 0) {
+#pragma unroll
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) ((uint32_t *)p)[i] = raw.w[i];
+    } else {
+        p[0] = raw.e[0];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) ((uint32_t *)(p + 1))[i] = __funnelshift_r(raw.w[i], raw.w[i + 1], 16);
+        p[7] = raw.e[7];
+    }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) swiglu_q8_kernel(const RowParams p) {
-    const size_t i = blockIdx.x;
-    const SwigluRow<T> row = {(const T *)p.a + i * p.a_stride, (const T *)p.b + i * p.b_stride};
-    row_q8(row, p);
+__device__ __forceinline__ void put8(int8_t *p, int n, const int (&q)[8]) {
+    const unsigned at = (unsigned)(uintptr_t)p;
+    if (n == 8 && (at & 3) == 0) {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            w[i] = (q[4 * i] & 255) | (q[4 * i + 1] & 255) << 8 | (q[4 * i + 2] & 255) << 16 | (uint32_t)q[4 * i + 3] << 24;
+        if ((at & 7) == 0) {
+            *(uint2 *)p = make_uint2(w[0], w[1]);
+        } else {
+            ((uint32_t *)p)[0] = w[0];
+            ((uint32_t *)p)[1] = w[1];
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < n) p[i] = (int8_t)q[i];
 }
 
-template <typename T> cudaError_t launch_norm(const RowParams &p, int rows, cudaStream_t st) {
-    norm_q8_kernel<T><<<rows, kRowThreads, 0, st>>>(p);
-    return cudaGetLastError();
+/* What the two kinds of rows have of their own: v of eight elements in 32
+ * bits, v of one in 64. */
+template <typename T> struct NormRow {
+    const T *x, *r;
+    T *h;
+    const float *w;
+    int n;
+    /* v: 2^-24; 127 / max|v|: 2 * 2^-24; their product: 2^-24; times 127: below 3.1e-5 */
+    static constexpr float kBorder = 4e-5f;
+    static constexpr bool kNorm = true;
+    __device__ NormRow(const RowParams &p)
+        : x((const T *)p.a + (size_t)blockIdx.x * p.a_stride),
+          r(p.b != nullptr ? (const T *)p.b + (size_t)blockIdx.x * p.b_stride : nullptr),
+          h(p.h != nullptr ? (T *)p.h + (size_t)blockIdx.x * p.h_stride : nullptr), w(p.w), n(p.n) {}
+    /* adds the residual, stores the sum, adds its squares to `sum` */
+    __device__ void load(int i, float (&v)[8], double &sum) const {
+        const int m = min(8, n - i);
+        get8(x + i, m, v);
+        float u[8];
+        if (r != nullptr) {
+            get8(r + i, m, u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = to_f32(from_f32<T>(__fadd_rn(v[j], u[j])));
+        }
+        if (h != nullptr) put8(h + i, m, v);
+        get8(w + i, m, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            sum = fma((double)v[j], (double)v[j], sum);
+            v[j] = __fmul_rn(v[j], u[j]);
+        }
+    }
+    /* the same v again, by the thread that loaded it */
+    __device__ void again(int i, float (&v)[8]) const {
+        const int m = min(8, n - i);
+        float u[8];
+        get8(h != nullptr ? (const T *)h + i : x + i, m, v);
+        get8(w + i, m, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], u[j]);
+    }
+    __device__ double v64(int i) const { return (double)to_f32(h != nullptr ? h[i] : x[i]) * (double)w[i]; }
+};
+
+template <typename T> struct SwigluRow {
+    const T *g, *u;
+    int n;
+    /* expf 2 ulp, 1 + e 0.5, __fdividef 2, the product 0.5 (5 * 2^-23), 127 / max|v| and the
+     * product with it 3 * 2^-24; times 127: below 1e-4 */
+    static constexpr float kBorder = 1.2e-4f;
+    static constexpr bool kNorm = false;
+    __device__ SwigluRow(const RowParams &p)
+        : g((const T *)p.a + (size_t)blockIdx.x * p.a_stride), u((const T *)p.b + (size_t)blockIdx.x * p.b_stride),
+          n(p.n) {}
+    __device__ void load(int i, float (&v)[8], double &) const {
+        const int m = min(8, n - i);
+        float up[8];
+        get8(g + i, m, v);
+        get8(u + i, m, up);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float gate = v[j];
+            v[j] = __fmul_rn(__fdividef(gate, 1.0f + expf(-gate)), up[j]);
+            /* there 1 + exp(-gate) leaves what __fdividef takes */
+            if (gate < -80.0f) v[j] = (float)silu64((double)gate, (double)up[j]);
+        }
+    }
+    __device__ void again(int i, float (&v)[8]) const {
+        double none;
+        load(i, v, none);
+    }
+    __device__ double v64(int i) const {
+        const float a = to_f32(g[i]), b = to_f32(u[i]);
+        return a == 0.0f || b == 0.0f ? (double)a * (double)b : silu64((double)a, (double)b);
+    }
+};
+
+/* Doubles that are not negative, NaN above all, order as their bits. */
+__device__ __forceinline__ unsigned long long abs_bits(double v) {
+    return (unsigned long long)__double_as_longlong(v) & 0x7fffffffffffffffull;
 }
-template <typename T> cudaError_t launch_swiglu(const RowParams &p, int rows, cudaStream_t st) {
-    swiglu_q8_kernel<T><<<rows, kRowThreads, 0, st>>>(p);
+
+__device__ __forceinline__ double of_bits(unsigned long long b) {
+    double v;
+    memcpy(&v, &b, sizeof v);
+    return v;
+}
+
+/* A row's statistics across the CTA. */
+struct RowShared {
+    double sums[32], sum;
+    unsigned tops[32];
+    unsigned long long top;
+};
+
+/* The largest |v| in 32 bits (as its bits) in every thread; the sum of `sum`
+ * in sh.sum after the next barrier. */
+template <bool kNorm> __device__ __forceinline__ unsigned row_top32(RowShared &sh, double sum, unsigned m) {
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (kNorm)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+        sh.tops[warp] = m;
+        sh.sums[warp] = sum;
+    }
+    if (threadIdx.x == 0) sh.top = 0;
+    __syncthreads();
+    if (kNorm && warp == 0) {
+        sum = lane < warps ? sh.sums[lane] : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) sh.sum = sum;
+    }
+    return __reduce_max_sync(0xffffffffu, lane < warps ? sh.tops[lane] : 0u);
+}
+
+/* Who may have the largest |v|: 64 bits decide (|error of v| < 1e-6). */
+__device__ __forceinline__ bool row_wide(float top32) { return !(top32 < kWideHi && top32 >= kWideLo); }
+__device__ __forceinline__ float row_least(float top32) { return row_wide(top32) ? 0.0f : top32 * (1.0f - 4e-6f); }
+
+/* A row's quantizer, once max|v| and the sum of squares are known. */
+template <typename Row> struct RowQuant {
+    double top;
+    float r32; /* 127 / top */
+    bool wide, fits; /* fits: fp32 holds the scale; else the row is NaN */
+
+    __device__ double factor(const RowParams &p, double sum) const {
+        return Row::kNorm ? 1.0 / sqrt(sum / p.n + (double)p.eps) : 1.0;
+    }
+    __device__ RowQuant(const RowParams &p, const RowShared &sh, bool wide_)
+        : top(of_bits(sh.top)), wide(wide_) {
+        r32 = __fdiv_rn(127.0f, (float)top);
+        float about = (float)top;
+        if (Row::kNorm) about *= rsqrtf((float)(sh.sum * (1.0 / p.n)) + p.eps);
+        fits = about < 1e38f || top == 0.0 || top * factor(p, sh.sum) <= (double)kFltMax;
+    }
+    __device__ void store(const RowParams &p, const Row &row, int i, const float (&v)[8]) const {
+        int out[8];
+        unsigned near = 0; /* elements next to a border */
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float t = __fmul_rn(v[j], r32), n = rintf(t);
+            if (!(fabsf(t - n) < 0.5f - Row::kBorder)) near |= 1u << j;
+            out[j] = (int)n;
+        }
+        if (wide) near = 255;
+        if (!fits || top == 0.0) {
+            near = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) out[j] = 0;
+        }
+        int8_t *q = p.q + (size_t)blockIdx.x * p.q_stride + i;
+        put8(q, min(8, p.n - i), out);
+        for (; near != 0; near &= near - 1) {
+            const int j = __ffs(near) - 1;
+            if (i + j < p.n) q[j] = (int8_t)round64(row.v64(i + j), top);
+        }
+    }
+    __device__ float scale(const RowParams &p, double sum) const {
+        return !fits ? __int_as_float(0x7fc00000) : top == 0.0 ? 0.0f : (float)(top * factor(p, sum) / 127.0);
+    }
+};
+
+/* One CTA a row, 8 kC elements a thread, which stay in registers between the
+ * statistics and the quantizer. */
+template <typename Row, int kC, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads) row_q8_kernel(const RowParams p) {
+    __shared__ RowShared sh;
+    const Row row(p);
+    float v[kC][8];
+    double sum = 0.0;
+    unsigned m = 0;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+        const int i = (c * blockDim.x + threadIdx.x) * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[c][j] = 0.0f;
+        if (i < p.n) row.load(i, v[c], sum);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(v[c][j])));
+    }
+    const float top32 = __uint_as_float(row_top32<Row::kNorm>(sh, sum, m)), least = row_least(top32);
+    if (!(__uint_as_float(m) < least)) {
+        unsigned long long best = 0;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            const int i = (c * blockDim.x + threadIdx.x) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i + j < p.n && !(fabsf(v[c][j]) < least)) best = max(best, abs_bits(row.v64(i + j)));
+        }
+        if (best) atomicMax(&sh.top, best);
+    }
+    __syncthreads();
+    const RowQuant<Row> rq(p, sh, row_wide(top32));
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+        const int i = (c * blockDim.x + threadIdx.x) * 8;
+        if (i < p.n) rq.store(p, row, i, v[c]);
+    }
+    if (threadIdx.x == 0) p.scale[blockIdx.x] = rq.scale(p, sh.sum);
+}
+
+/* Rows longer than a CTA's registers hold: every element is visited again. */
+constexpr int kLongThreads = 512;
+template <typename Row> __global__ void __launch_bounds__(kLongThreads) row_q8_long_kernel(const RowParams p) {
+    __shared__ RowShared sh;
+    const Row row(p);
+    double sum = 0.0;
+    unsigned m = 0;
+    float v[8];
+    for (int i = threadIdx.x * 8; i < p.n; i += kLongThreads * 8) {
+        row.load(i, v, sum);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j < p.n) m = max(m, __float_as_uint(fabsf(v[j])));
+    }
+    const float top32 = __uint_as_float(row_top32<Row::kNorm>(sh, sum, m)), least = row_least(top32);
+    if (!(__uint_as_float(m) < least)) {
+        unsigned long long best = 0;
+        for (int i = threadIdx.x * 8; i < p.n; i += kLongThreads * 8) {
+            row.again(i, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i + j < p.n && !(fabsf(v[j]) < least)) best = max(best, abs_bits(row.v64(i + j)));
+        }
+        if (best) atomicMax(&sh.top, best);
+    }
+    __syncthreads();
+    const RowQuant<Row> rq(p, sh, row_wide(top32));
+    for (int i = threadIdx.x * 8; i < p.n; i += kLongThreads * 8) {
+        row.again(i, v);
+        rq.store(p, row, i, v);
+    }
+    if (threadIdx.x == 0) p.scale[blockIdx.x] = rq.scale(p, sh.sum);
+}
+
+template <typename Row> cudaError_t launch_rows(const RowParams &p, int rows, cudaStream_t st) {
+    const int eights = (p.n + 7) / 8;
+    auto threads = [&](int c) { return ((eights + c - 1) / c + 31) / 32 * 32; };
+    if (eights <= 1024)
+        row_q8_kernel<Row, 1, 1024><<<rows, threads(1), 0, st>>>(p);
+    else if (eights <= 2048)
+        row_q8_kernel<Row, 2, 1024><<<rows, threads(2), 0, st>>>(p);
+    else if (eights <= 4 * 640)
+        row_q8_kernel<Row, 4, 640><<<rows, threads(4), 0, st>>>(p);
+    else
+        row_q8_long_kernel<Row><<<rows, kLongThreads, 0, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -247,9 +427,9 @@ int lal_tail_add_rms_norm_q8(const void *d_x, int64_t x_stride, const void *d_re
     const RowParams p = {d_x, d_residual, d_h, d_norm_w, x_stride, residual_stride, h_stride, q_stride,
                          n_embd, eps, d_q, d_scale};
     cudaStream_t st = (cudaStream_t)stream;
-    return launched(op, dtype == LAL_TAIL_F32    ? launch_norm<float>(p, rows, st)
-                        : dtype == LAL_TAIL_BF16 ? launch_norm<__nv_bfloat16>(p, rows, st)
-                                                 : launch_norm<__half>(p, rows, st));
+    return launched(op, dtype == LAL_TAIL_F32    ? launch_rows<NormRow<float>>(p, rows, st)
+                        : dtype == LAL_TAIL_BF16 ? launch_rows<NormRow<__nv_bfloat16>>(p, rows, st)
+                                                 : launch_rows<NormRow<__half>>(p, rows, st));
 }
 
 int lal_tail_swiglu_q8(const void *d_gate, int64_t gate_stride, const void *d_up, int64_t up_stride,
@@ -277,9 +457,9 @@ int lal_tail_swiglu_q8(const void *d_gate, int64_t gate_stride, const void *d_up
     const RowParams p = {d_gate, d_up, nullptr, nullptr, gate_stride, up_stride, 0, q_stride,
                          n, 0.0f, d_q, d_scale};
     cudaStream_t st = (cudaStream_t)stream;
-    return launched(op, dtype == LAL_TAIL_F32    ? launch_swiglu<float>(p, rows, st)
-                        : dtype == LAL_TAIL_BF16 ? launch_swiglu<__nv_bfloat16>(p, rows, st)
-                                                 : launch_swiglu<__half>(p, rows, st));
+    return launched(op, dtype == LAL_TAIL_F32    ? launch_rows<SwigluRow<float>>(p, rows, st)
+                        : dtype == LAL_TAIL_BF16 ? launch_rows<SwigluRow<__nv_bfloat16>>(p, rows, st)
+                                                 : launch_rows<SwigluRow<__half>>(p, rows, st));
 }
 
 }  // extern "C"
