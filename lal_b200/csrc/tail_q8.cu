@@ -18,6 +18,7 @@
  */
 #include "tail_layer.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -34,6 +35,8 @@ struct RowParams {
     float eps;
     int8_t *q;
     float *scale;
+    int parts;   /* CTAs a row */
+    float inv_n; /* 1 / n */
 };
 
 /* What few elements need, out of line: inlined for each of a thread's elements
@@ -112,24 +115,19 @@ template <typename T> __device__ __forceinline__ void put8(T *p, int n, const fl
     }
 }
 
-__device__ __forceinline__ void put8(int8_t *p, int n, const int (&q)[8]) {
+/* n of eight bytes */
+__device__ __forceinline__ void put_q8(int8_t *p, int n, const uint32_t (&w)[2]) {
     const unsigned at = (unsigned)(uintptr_t)p;
-    if (n == 8 && (at & 3) == 0) {
-        uint32_t w[2];
+    if (n == 8 && (at & 7) == 0) {
+        *(uint2 *)p = make_uint2(w[0], w[1]);
+    } else if (n == 8 && (at & 3) == 0) {
+        ((uint32_t *)p)[0] = w[0];
+        ((uint32_t *)p)[1] = w[1];
+    } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            w[i] = (q[4 * i] & 255) | (q[4 * i + 1] & 255) << 8 | (q[4 * i + 2] & 255) << 16 | (uint32_t)q[4 * i + 3] << 24;
-        if ((at & 7) == 0) {
-            *(uint2 *)p = make_uint2(w[0], w[1]);
-        } else {
-            ((uint32_t *)p)[0] = w[0];
-            ((uint32_t *)p)[1] = w[1];
-        }
-        return;
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < n) p[i] = (int8_t)q[i];
 }
 
 /* What the two kinds of rows have of their own: v of eight elements in 32
@@ -142,10 +140,10 @@ template <typename T> struct NormRow {
     /* v: 2^-24; 127 / max|v|: 2 * 2^-24; their product: 2^-24; times 127: below 3.1e-5 */
     static constexpr float kBorder = 4e-5f;
     static constexpr bool kNorm = true;
-    __device__ NormRow(const RowParams &p)
-        : x((const T *)p.a + (size_t)blockIdx.x * p.a_stride),
-          r(p.b != nullptr ? (const T *)p.b + (size_t)blockIdx.x * p.b_stride : nullptr),
-          h(p.h != nullptr ? (T *)p.h + (size_t)blockIdx.x * p.h_stride : nullptr), w(p.w), n(p.n) {}
+    __device__ NormRow(const RowParams &p, int at)
+        : x((const T *)p.a + (size_t)at * p.a_stride),
+          r(p.b != nullptr ? (const T *)p.b + (size_t)at * p.b_stride : nullptr),
+          h(p.h != nullptr ? (T *)p.h + (size_t)at * p.h_stride : nullptr), w(p.w), n(p.n) {}
     /* adds the residual, stores the sum, adds its squares to `sum` */
     __device__ void load(int i, float (&v)[8], double &sum) const {
         const int m = min(8, n - i);
@@ -183,8 +181,8 @@ template <typename T> struct SwigluRow {
      * product with it 3 * 2^-24; times 127: below 1e-4 */
     static constexpr float kBorder = 1.2e-4f;
     static constexpr bool kNorm = false;
-    __device__ SwigluRow(const RowParams &p)
-        : g((const T *)p.a + (size_t)blockIdx.x * p.a_stride), u((const T *)p.b + (size_t)blockIdx.x * p.b_stride),
+    __device__ SwigluRow(const RowParams &p, int at)
+        : g((const T *)p.a + (size_t)at * p.a_stride), u((const T *)p.b + (size_t)at * p.b_stride),
           n(p.n) {}
     __device__ void load(int i, float (&v)[8], double &) const {
         const int m = min(8, n - i);
@@ -220,168 +218,245 @@ __device__ __forceinline__ double of_bits(unsigned long long b) {
     return v;
 }
 
-/* A row's statistics across the CTA. */
+/* max with NaN above all */
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float v;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
+    return v;
+}
+
+constexpr int kMaxParts = 8; /* CTAs of a row: a portable cluster */
+
+/* A row's statistics: across a CTA, then across the CTAs of the row. */
 struct RowShared {
-    double sums[32], sum;
+    double sums[32];
     unsigned tops[32];
-    unsigned long long top;
+    unsigned long long top; /* max|v| of this CTA's part, in 64 bits */
+    double part_sum[kMaxParts];
+    unsigned long long part_top[kMaxParts];
 };
 
-/* The largest |v| in 32 bits (as its bits) in every thread; the sum of `sum`
- * in sh.sum after the next barrier. */
-template <bool kNorm> __device__ __forceinline__ unsigned row_top32(RowShared &sh, double sum, unsigned m) {
+__device__ __forceinline__ bool row_wide(float top32) { return !(top32 < kWideHi && top32 >= kWideLo); }
+
+/* The row's max|v| in 64 bits and sum of squares, in every thread, from each
+ * thread's largest |v| in 32 bits `m` and `sum`.  Only elements whose |v| may
+ * be the largest (its error is below 1e-6) are computed in 64 bits; `best(least)`
+ * is their largest, as bits, of the thread's elements not below `least`. */
+template <bool kNorm, bool kCluster, typename Best>
+__device__ __forceinline__ double row_stat(RowShared &sh, int parts, int part, float m, double &sum, Best best) {
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    m = __reduce_max_sync(0xffffffffu, m);
+    const unsigned top_warp = __reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7fffffffu);
     if (kNorm)
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
-        sh.tops[warp] = m;
+        sh.tops[warp] = top_warp;
         sh.sums[warp] = sum;
     }
     if (threadIdx.x == 0) sh.top = 0;
     __syncthreads();
+    const float top32 = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? sh.tops[lane] : 0u));
+    const float least = row_wide(top32) ? 0.0f : top32 * (1.0f - 4e-6f);
+    if (!(m < least)) {
+        const unsigned long long b = best(least);
+        if (b) atomicMax(&sh.top, b);
+    }
     if (kNorm && warp == 0) {
         sum = lane < warps ? sh.sums[lane] : 0.0;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) sh.sum = sum;
+        if (lane == 0) sh.part_sum[part] = sum;
     }
-    return __reduce_max_sync(0xffffffffu, lane < warps ? sh.tops[lane] : 0u);
+    __syncthreads();
+    if (!kCluster) {
+        if (kNorm) sum = sh.part_sum[0];
+        return of_bits(sh.top);
+    }
+    /* to every CTA of the row, once all have begun; none leaves before all have written */
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (threadIdx.x < parts) {
+        uint32_t at;
+        const unsigned long long top = sh.top;
+        const uint32_t here = (uint32_t)__cvta_generic_to_shared(&sh.part_top[part]);
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(here), "r"(threadIdx.x));
+        asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(at), "l"(top) : "memory");
+        if (kNorm) {
+            const uint32_t here_s = (uint32_t)__cvta_generic_to_shared(&sh.part_sum[part]);
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(here_s), "r"(threadIdx.x));
+            asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(at), "l"(__double_as_longlong(sh.part_sum[part])) : "memory");
+        }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    unsigned long long top = 0;
+    if (kNorm) sum = 0.0;
+    for (int i = 0; i < parts; ++i) {
+        top = max(top, sh.part_top[i]);
+        if (kNorm) sum += sh.part_sum[i];
+    }
+    return of_bits(top);
 }
-
-/* Who may have the largest |v|: 64 bits decide (|error of v| < 1e-6). */
-__device__ __forceinline__ bool row_wide(float top32) { return !(top32 < kWideHi && top32 >= kWideLo); }
-__device__ __forceinline__ float row_least(float top32) { return row_wide(top32) ? 0.0f : top32 * (1.0f - 4e-6f); }
 
 /* A row's quantizer, once max|v| and the sum of squares are known. */
 template <typename Row> struct RowQuant {
-    double top;
+    double top, sum;
     float r32; /* 127 / top */
     bool wide, fits; /* fits: fp32 holds the scale; else the row is NaN */
 
-    __device__ double factor(const RowParams &p, double sum) const {
+    __device__ double factor(const RowParams &p) const {
         return Row::kNorm ? 1.0 / sqrt(sum / p.n + (double)p.eps) : 1.0;
     }
-    __device__ RowQuant(const RowParams &p, const RowShared &sh, bool wide_)
-        : top(of_bits(sh.top)), wide(wide_) {
-        r32 = __fdiv_rn(127.0f, (float)top);
+    __device__ RowQuant(const RowParams &p, double top_, double sum_) : top(top_), sum(sum_) {
         float about = (float)top;
-        if (Row::kNorm) about *= rsqrtf((float)(sh.sum * (1.0 / p.n)) + p.eps);
-        fits = about < 1e38f || top == 0.0 || top * factor(p, sh.sum) <= (double)kFltMax;
+        wide = row_wide(about);
+        r32 = __fdiv_rn(127.0f, about);
+        if (Row::kNorm) about *= rsqrtf((float)sum * p.inv_n + p.eps);
+        fits = about < 1e38f || top == 0.0 || top * factor(p) <= (double)kFltMax;
     }
-    __device__ void store(const RowParams &p, const Row &row, int i, const float (&v)[8]) const {
-        int out[8];
-        unsigned near = 0; /* elements next to a border */
+    /* q of the eight elements from i on */
+    __device__ void store(const RowParams &p, const Row &row, int8_t *q, int i, const float (&v)[8]) const {
+        constexpr float kRound = 12582912.0f; /* 1.5 * 2^23: added, it leaves the nearest integer in the low bits */
+        float u[8], far = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float t = __fmul_rn(v[j], r32), n = rintf(t);
-            if (!(fabsf(t - n) < 0.5f - Row::kBorder)) near |= 1u << j;
-            out[j] = (int)n;
+            const float t = __fmul_rn(v[j], r32);
+            u[j] = __fadd_rn(t, kRound);
+            far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(u[j], kRound))));
         }
-        if (wide) near = 255;
-        if (!fits || top == 0.0) {
-            near = 0;
+        uint32_t w[2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) out[j] = 0;
-        }
-        int8_t *q = p.q + (size_t)blockIdx.x * p.q_stride + i;
-        put8(q, min(8, p.n - i), out);
-        for (; near != 0; near &= near - 1) {
-            const int j = __ffs(near) - 1;
-            if (i + j < p.n) q[j] = (int8_t)round64(row.v64(i + j), top);
+        for (int h = 0; h < 2; ++h)
+            w[h] = __byte_perm(__byte_perm(__float_as_uint(u[4 * h]), __float_as_uint(u[4 * h + 1]), 0x0040),
+                               __byte_perm(__float_as_uint(u[4 * h + 2]), __float_as_uint(u[4 * h + 3]), 0x0040), 0x5410);
+        const bool none = !fits || top == 0.0;
+        if (none) w[0] = w[1] = 0;
+        const int n = min(8, p.n - i);
+        put_q8(q + i, n, w);
+        if ((wide || !(far < 0.5f - Row::kBorder)) && !none) { /* next to a border: 64 bits decide */
+#pragma unroll 1
+            for (int j = 0; j < n; ++j) {
+                float t = 0.5f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k == j) t = __fmul_rn(v[k], r32);
+                if (wide || !(fabsf(t - rintf(t)) < 0.5f - Row::kBorder)) q[i + j] = (int8_t)round64(row.v64(i + j), top);
+            }
         }
     }
-    __device__ float scale(const RowParams &p, double sum) const {
-        return !fits ? __int_as_float(0x7fc00000) : top == 0.0 ? 0.0f : (float)(top * factor(p, sum) / 127.0);
+    __device__ float scale(const RowParams &p) const {
+        return !fits ? __int_as_float(0x7fc00000) : top == 0.0 ? 0.0f : (float)(top * factor(p) / 127.0);
     }
 };
 
-/* One CTA a row, 8 kC elements a thread, which stay in registers between the
- * statistics and the quantizer. */
-template <typename Row, int kC, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads) row_q8_kernel(const RowParams p) {
+/* A row a CTA, or (kCluster) a cluster: 8 kC elements a thread, which stay in
+ * registers between the statistics and the quantizer. */
+template <typename Row, int kC, int kMaxThreads, int kMinCtas, bool kCluster>
+__global__ void __launch_bounds__(kMaxThreads, kMinCtas) row_q8_kernel(const RowParams p) {
     __shared__ RowShared sh;
-    const Row row(p);
-    float v[kC][8];
+    const int parts = kCluster ? p.parts : 1, part = kCluster ? blockIdx.x % parts : 0;
+    const int at = kCluster ? blockIdx.x / parts : blockIdx.x;
+    if (kCluster) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const Row row(p, at);
+    const int first = part * blockDim.x * (8 * kC);
+    float v[kC][8], m = 0.0f;
     double sum = 0.0;
-    unsigned m = 0;
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-        const int i = (c * blockDim.x + threadIdx.x) * 8;
+        const int i = first + (c * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[c][j] = 0.0f;
         if (i < p.n) row.load(i, v[c], sum);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(v[c][j])));
     }
-    const float top32 = __uint_as_float(row_top32<Row::kNorm>(sh, sum, m)), least = row_least(top32);
-    if (!(__uint_as_float(m) < least)) {
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[c][j]));
+    const double top = row_stat<Row::kNorm, kCluster>(sh, parts, part, m, sum, [&](float least) {
         unsigned long long best = 0;
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
-            const int i = (c * blockDim.x + threadIdx.x) * 8;
+            const int i = first + (c * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (i + j < p.n && !(fabsf(v[c][j]) < least)) best = max(best, abs_bits(row.v64(i + j)));
         }
-        if (best) atomicMax(&sh.top, best);
-    }
-    __syncthreads();
-    const RowQuant<Row> rq(p, sh, row_wide(top32));
+        return best;
+    });
+    const RowQuant<Row> rq(p, top, sum);
+    int8_t *q = p.q + (size_t)at * p.q_stride;
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-        const int i = (c * blockDim.x + threadIdx.x) * 8;
-        if (i < p.n) rq.store(p, row, i, v[c]);
+        const int i = first + (c * blockDim.x + threadIdx.x) * 8;
+        if (i < p.n) rq.store(p, row, q, i, v[c]);
     }
-    if (threadIdx.x == 0) p.scale[blockIdx.x] = rq.scale(p, sh.sum);
+    if (part == 0 && threadIdx.x == 0) p.scale[at] = rq.scale(p);
 }
 
-/* Rows longer than a CTA's registers hold: every element is visited again. */
+/* Rows longer than that: one CTA, and every element is visited again. */
 constexpr int kLongThreads = 512;
 template <typename Row> __global__ void __launch_bounds__(kLongThreads) row_q8_long_kernel(const RowParams p) {
     __shared__ RowShared sh;
-    const Row row(p);
+    const Row row(p, blockIdx.x);
     double sum = 0.0;
-    unsigned m = 0;
-    float v[8];
+    float v[8], m = 0.0f;
     for (int i = threadIdx.x * 8; i < p.n; i += kLongThreads * 8) {
         row.load(i, v, sum);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i + j < p.n) m = max(m, __float_as_uint(fabsf(v[j])));
+        for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
     }
-    const float top32 = __uint_as_float(row_top32<Row::kNorm>(sh, sum, m)), least = row_least(top32);
-    if (!(__uint_as_float(m) < least)) {
+    const double top = row_stat<Row::kNorm, false>(sh, 1, 0, m, sum, [&](float least) {
         unsigned long long best = 0;
         for (int i = threadIdx.x * 8; i < p.n; i += kLongThreads * 8) {
             row.again(i, v);
-#pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (i + j < p.n && !(fabsf(v[j]) < least)) best = max(best, abs_bits(row.v64(i + j)));
         }
-        if (best) atomicMax(&sh.top, best);
-    }
-    __syncthreads();
-    const RowQuant<Row> rq(p, sh, row_wide(top32));
+        return best;
+    });
+    const RowQuant<Row> rq(p, top, sum);
+    int8_t *q = p.q + (size_t)blockIdx.x * p.q_stride;
     for (int i = threadIdx.x * 8; i < p.n; i += kLongThreads * 8) {
         row.again(i, v);
-        rq.store(p, row, i, v);
+        rq.store(p, row, q, i, v);
     }
-    if (threadIdx.x == 0) p.scale[blockIdx.x] = rq.scale(p, sh.sum);
+    if (threadIdx.x == 0) p.scale[blockIdx.x] = rq.scale(p);
 }
 
-template <typename Row> cudaError_t launch_rows(const RowParams &p, int rows, cudaStream_t st) {
+template <typename Row, int kC, int kMaxThreads, int kMinCtas>
+cudaError_t launch_parts(RowParams p, int rows, int parts, cudaStream_t st) {
     const int eights = (p.n + 7) / 8;
-    auto threads = [&](int c) { return ((eights + c - 1) / c + 31) / 32 * 32; };
-    if (eights <= 1024)
-        row_q8_kernel<Row, 1, 1024><<<rows, threads(1), 0, st>>>(p);
-    else if (eights <= 2048)
-        row_q8_kernel<Row, 2, 1024><<<rows, threads(2), 0, st>>>(p);
-    else if (eights <= 4 * 640)
-        row_q8_kernel<Row, 4, 640><<<rows, threads(4), 0, st>>>(p);
-    else
-        row_q8_long_kernel<Row><<<rows, kLongThreads, 0, st>>>(p);
+    const int threads = ((eights + parts * kC - 1) / (parts * kC) + 31) / 32 * 32;
+    p.parts = parts;
+    if (parts == 1) {
+        row_q8_kernel<Row, kC, kMaxThreads, kMinCtas, false><<<rows, threads, 0, st>>>(p);
+        return cudaGetLastError();
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * parts));
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, row_q8_kernel<Row, kC, kMaxThreads, kMinCtas, true>, p);
+}
+
+constexpr int kFewN = 8192, kFewPart = 2048;
+template <typename Row> cudaError_t launch_rows(RowParams p, int rows, int num_sms, cudaStream_t st) {
+    p.inv_n = 1.0f / (float)p.n;
+    /* Few rows: a thread takes 8 elements, and a long row is spread over as
+     * many SMs as a cluster has.  Many: 16 elements, and no more CTAs a row
+     * than its registers need. */
+    if (rows < 2 * num_sms) {
+        if (p.n <= kFewN) return launch_parts<Row, 1, 1024, 1>(p, rows, 1, st);
+        if (p.n <= kMaxParts * 8192) return launch_parts<Row, 1, 1024, 1>(p, rows, std::min(kMaxParts, (p.n + kFewPart - 1) / kFewPart), st);
+    } else if (p.n <= kMaxParts * 8192 && rows <= 0x7fffffff / kMaxParts) {
+        return launch_parts<Row, 2, 512, 2>(p, rows, (p.n + 8191) / 8192, st);
+    }
+    row_q8_long_kernel<Row><<<rows, kLongThreads, 0, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -425,11 +500,11 @@ int lal_tail_add_rms_norm_q8(const void *d_x, int64_t x_stride, const void *d_re
     CallDevice dev;
     if (const int rc = dev.enter(op, names, ptrs, 6)) return rc;
     const RowParams p = {d_x, d_residual, d_h, d_norm_w, x_stride, residual_stride, h_stride, q_stride,
-                         n_embd, eps, d_q, d_scale};
+                         n_embd, eps, d_q, d_scale, 1, 0.0f};
     cudaStream_t st = (cudaStream_t)stream;
-    return launched(op, dtype == LAL_TAIL_F32    ? launch_rows<NormRow<float>>(p, rows, st)
-                        : dtype == LAL_TAIL_BF16 ? launch_rows<NormRow<__nv_bfloat16>>(p, rows, st)
-                                                 : launch_rows<NormRow<__half>>(p, rows, st));
+    return launched(op, dtype == LAL_TAIL_F32    ? launch_rows<NormRow<float>>(p, rows, dev.num_sms(), st)
+                        : dtype == LAL_TAIL_BF16 ? launch_rows<NormRow<__nv_bfloat16>>(p, rows, dev.num_sms(), st)
+                                                 : launch_rows<NormRow<__half>>(p, rows, dev.num_sms(), st));
 }
 
 int lal_tail_swiglu_q8(const void *d_gate, int64_t gate_stride, const void *d_up, int64_t up_stride,
@@ -455,11 +530,11 @@ int lal_tail_swiglu_q8(const void *d_gate, int64_t gate_stride, const void *d_up
     CallDevice dev;
     if (const int rc = dev.enter(op, names, ptrs, 4)) return rc;
     const RowParams p = {d_gate, d_up, nullptr, nullptr, gate_stride, up_stride, 0, q_stride,
-                         n, 0.0f, d_q, d_scale};
+                         n, 0.0f, d_q, d_scale, 1, 0.0f};
     cudaStream_t st = (cudaStream_t)stream;
-    return launched(op, dtype == LAL_TAIL_F32    ? launch_rows<SwigluRow<float>>(p, rows, st)
-                        : dtype == LAL_TAIL_BF16 ? launch_rows<SwigluRow<__nv_bfloat16>>(p, rows, st)
-                                                 : launch_rows<SwigluRow<__half>>(p, rows, st));
+    return launched(op, dtype == LAL_TAIL_F32    ? launch_rows<SwigluRow<float>>(p, rows, dev.num_sms(), st)
+                        : dtype == LAL_TAIL_BF16 ? launch_rows<SwigluRow<__nv_bfloat16>>(p, rows, dev.num_sms(), st)
+                                                 : launch_rows<SwigluRow<__half>>(p, rows, dev.num_sms(), st));
 }
 
 }  // extern "C"
