@@ -12,13 +12,13 @@
  *   symmetric     w = s * (q - 8)
  *   with minimum  w = s * q + m
  */
+#include "tail_device.cuh"
 #include "tail_layer.h"
 
 #include <algorithm>
 #include <type_traits>
 
-using namespace lal;
-
+namespace lal {
 namespace {
 
 constexpr int kQ4Block = 32; /* columns of a 16-byte block */
@@ -260,9 +260,6 @@ constexpr int kMmaSmem = 113 * 1024 - 1024; /* two CTAs an SM */
 static_assert(kMmaWarps * 3 * (kStageA + kStageS + 8 * kStageXRow) <= kMmaSmem, "up to eight streams, three stages");
 static_assert(kMmaWarps * 4 * (kStageA + kStageS + 3 * kStageXRow) <= kMmaSmem, "up to three streams, four stages");
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return (uint32_t)__cvta_generic_to_shared(p);
-}
 /* 16 (or 4) bytes to shared memory, the last 16 - n of them zeros */
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int n) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
@@ -639,7 +636,432 @@ cudaError_t launch_mma(const MatvecParams &p, int num_sms, cudaStream_t st) {
     return cudaGetLastError();
 }
 
+/* ---- nine streams and more: tcgen05.mma kind::i8 ----
+ *
+ * A CTA takes tiles of 128 rows by up to kN streams.  The weights are the A
+ * operand and lie in tensor memory: a thread of the four unpacking warps has a
+ * row, reads its 16-byte blocks from a ring of its warp's own (cp.async) and
+ * stores 16 (q - 8) as int8, eight columns of tensor memory a block.  The
+ * vectors are the B operand, in shared memory with the 128-byte swizzle.  One
+ * thread issues the products, a group of columns at a time into one of kD
+ * accumulators; eight warps read a finished one (int32, exact), scale it by
+ * the row's scale of the group and add it in fp32 registers, while the next
+ * groups are multiplied.  So every scale is applied in fp32, the weights are
+ * read once, and only the unpacked weights' 8-bit form is ever written on the
+ * chip.  With few tiles, the K range of a tile is split over a cluster of
+ * CTAs, whose sums are exchanged and added in order over distributed shared
+ * memory.
+ *
+ * Every wait is bounded; one that runs out makes the tile's results NaN. */
+constexpr int kTcUnpack = 4, kTcEpi = 8, kTcLoad = 2;
+constexpr int kTcWarps = kTcUnpack + kTcEpi + 1 + kTcLoad;
+constexpr int kTcD = 4;        /* accumulators */
+constexpr int kTcWDepth = 6;   /* stages of a warp's weight ring */
+constexpr int kTcXDepth = 4;   /* stages of the vectors */
+constexpr int kTcWStage = 32 * kStageBlocks * 16;
+constexpr int kTcMaxSplit = 8;
+
+struct TcShared {
+    uint64_t a_full[2], a_empty[2], x_full[kTcXDepth], x_empty[kTcXDepth], d_full[kTcD], d_empty[kTcD], drain;
+    uint32_t tmem;
+    int abort, never;
+};
+
+__host__ __device__ constexpr int tc_x_stage(int n) { return n * kStageBlocks * 32; }
+__host__ __device__ constexpr int tc_sum_bytes(int n, int group) { return kTcXDepth * (kStageBlocks * 32 / group) * n * 4; }
+template <int kN, int kGroup, bool kMin> constexpr int tc_smem() {
+    return 1024 + kTcUnpack * kTcWDepth * kTcWStage + kTcXDepth * tc_x_stage(kN) + (kMin ? tc_sum_bytes(kN, kGroup) : 0);
+}
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+/* arrive on bar when every tcgen05.mma this thread issued before has completed */
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+/* D[tensor memory] (+)= A[tensor memory] * B[shared memory]^T, int8 x int8 -> int32 */
+__device__ __forceinline__ void tc_mma_i8_ta(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+                 "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate), "r"(0));
+}
+/* Shared-memory descriptor of rows of 128 bytes with the 128-byte swizzle
+ * (8-row groups 1024 bytes apart); 32 bytes further is the next K step. */
+__device__ __forceinline__ uint64_t tc_desc(uint32_t at) {
+    return (uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+/* int32 accumulators, signed int8 operands, both K-major, 128 rows by n */
+__device__ constexpr uint32_t tc_idesc(int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void tc_store8(uint32_t at, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tc_load8(uint32_t at, int *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(at));
+}
+
+template <int kN, int kGroup, bool kMin>
+__global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecParams p, int splits, int x_base) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ TcShared sh;
+    constexpr int kPer = kGroup / kQ4Block, kGroups = kStageBlocks / kPer; /* blocks a group, groups a stage */
+    constexpr int kHalf = kN / 2;                                          /* streams of an epilogue warp */
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t *xring = smem;                                      /* kTcXDepth stages of two swizzled tiles */
+    uint8_t *wring = xring + kTcXDepth * tc_x_stage(kN);        /* of each unpacking warp */
+    float *xsums = (float *)(wring + kTcUnpack * kTcWDepth * kTcWStage); /* [kTcXDepth][kGroups][kN] */
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int *abort_flag = &sh.abort, *never = &sh.never;
+    const int b0 = x_base + blockIdx.y * kN, nx = min(kN, p.streams - b0);
+    const int nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
+    const int all = (nb + kStageBlocks - 1) / kStageBlocks; /* stages of a row */
+    const int tiles = (p.rows + 127) / 128;
+    /* this CTA's tiles, and its stages of each */
+    const int split = (int)(blockIdx.x % splits), tile0 = (int)(blockIdx.x / splits), tile_step = (int)(gridDim.x / splits);
+    const int st0 = (int)((long long)all * split / splits), st1 = (int)((long long)all * (split + 1) / splits);
+    const int my_tiles = tile0 < tiles ? (tiles - 1 - tile0) / tile_step + 1 : 0;
+    const int per = st1 - st0, total = my_tiles * per;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) mbar_init(&sh.a_full[i], kTcUnpack), mbar_init(&sh.a_empty[i], 1);
+        for (int i = 0; i < kTcXDepth; ++i)
+            mbar_init(&sh.x_full[i], kTcLoad), mbar_init(&sh.x_empty[i], 1 + (kMin ? kTcEpi : 0));
+        for (int i = 0; i < kTcD; ++i) mbar_init(&sh.d_full[i], 1), mbar_init(&sh.d_empty[i], kTcEpi);
+        mbar_init(&sh.drain, 1);
+        sh.abort = sh.never = 0;
+        mbar_fence_init();
+    }
+    constexpr int kCols = 128 + kTcD * kN <= 256 ? 256 : 512;
+    if (warp == kTcUnpack + kTcEpi) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(kCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem, tmem_d = tmem + 128; /* two A operands of 64 columns, then the accumulators */
+
+    float acc[kHalf]; /* of an epilogue thread */
+
+    if (warp < kTcUnpack) {
+        /* ---- weights: 4 bits in global memory -> int8 in tensor memory ---- */
+        uint8_t *ring = wring + warp * kTcWDepth * kTcWStage;
+        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+        auto load = [&](int it) {
+            if (it < total) {
+                const int row0 = (tile0 + it / per * tile_step) * 128 + warp * 32, k0 = (st0 + it % per) * kStageBlocks;
+                const bool in = k0 + (lane & 7) < nb;
+                const uint32_t dst = smem_u32(ring + it % kTcWDepth * kTcWStage) + (lane >> 3) * 128;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int r = (lane >> 3) + 4 * j;
+                    const uint8_t *src = p.q + ((size_t)min(row0 + r, p.rows - 1) * nb + (in ? k0 + (lane & 7) : 0)) * 16;
+                    cp_async16(dst + j * 512 + (((lane & 7) ^ (r & 7)) << 4), src, in ? 16 : 0);
+                }
+            }
+            cp_async_commit();
+        };
+        for (int i = 0; i < kTcWDepth - 1; ++i) load(i);
+        for (int it = 0; it < total; ++it) {
+            cp_async_wait<kTcWDepth - 2>();
+            __syncwarp();
+            load(it + kTcWDepth - 1);
+            const int buf = it & 1;
+            if (it >= 2 && !mbar_wait(&sh.a_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag)) {
+                *abort_flag = 1;
+                break;
+            }
+            __syncwarp();
+            tc_fence_after();
+            const uint8_t *row = ring + it % kTcWDepth * kTcWStage + lane * 128;
+#pragma unroll
+            for (int k = 0; k < kStageBlocks; ++k) {
+                const uint4 v = *(const uint4 *)(row + ((k ^ (lane & 7)) << 4));
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                uint32_t o[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[i] = ((w[i] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+                    o[4 + i] = (w[i] & 0xf0f0f0f0u) ^ 0x80808080u;
+                }
+                tc_store8(lanes + buf * 64 + k * 8, o);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.a_full[buf]);
+        }
+        cp_async_wait<0>();
+    } else if (warp < kTcUnpack + kTcEpi) {
+        /* ---- accumulators: scaled and added ---- */
+        const int quad = warp & 3, half = (warp - kTcUnpack) >> 2;
+        const uint32_t lanes = tmem_d + ((uint32_t)(quad * 32) << 16) + half * kHalf;
+        /* a row's scales (and minima) of a stage, one load where all rows' are aligned to it */
+        using Pack = std::conditional_t<kGroups == 8, uint4, std::conditional_t<kGroups == 4, uint2, uint32_t>>;
+        union Row {
+            Pack all;
+            unsigned short one[kGroups];
+            __device__ Row() {}
+        } scale, low, scale_next, low_next;
+        const bool s_aligned =
+            (((uintptr_t)p.scale | (kMin ? (uintptr_t)p.min : 0) | (uintptr_t)(groups * 2)) & (2 * kGroups - 1)) == 0;
+        auto load_scales = [&](int it) {
+            const int row = min((tile0 + it / per * tile_step) * 128 + quad * 32 + lane, p.rows - 1);
+            const int g0 = (st0 + it % per) * kGroups;
+            const size_t at = (size_t)row * groups + g0;
+            if (s_aligned && g0 + kGroups <= groups) {
+                scale_next.all = __ldg((const Pack *)(p.scale + at));
+                if (kMin) low_next.all = __ldg((const Pack *)(p.min + at));
+            } else {
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i) {
+                    scale_next.one[i] = g0 + i < groups ? __ldg((const unsigned short *)p.scale + at + i) : 0;
+                    if (kMin) low_next.one[i] = g0 + i < groups ? __ldg((const unsigned short *)p.min + at + i) : 0;
+                }
+            }
+        };
+        if (total > 0) load_scales(0);
+        bool ok = true;
+        for (int it = 0, d = 0; it < total; ++it) {
+            if (it % per == 0)
+#pragma unroll
+                for (int j = 0; j < kHalf; ++j) acc[j] = 0.0f;
+            scale.all = scale_next.all;
+            if (kMin) low.all = low_next.all;
+            if (it + 1 < total) load_scales(it + 1);
+            const int xs = it % kTcXDepth;
+            if (kMin && ok && !mbar_wait(&sh.x_full[xs], (it / kTcXDepth) & 1, abort_flag)) ok = false;
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr, ++d) {
+                const int buf = d % kTcD;
+                if (ok && !mbar_wait(&sh.d_full[buf], (d / kTcD) & 1, abort_flag)) ok = false;
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    *abort_flag = 1;
+                    break;
+                }
+                tc_fence_after();
+                int c[kHalf];
+#pragma unroll
+                for (int j = 0; j < kHalf; j += 8) tc_load8(lanes + buf * kN + j, c + j);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.d_empty[buf]);
+                const float s = __half2float(__ushort_as_half(scale.one[gr]));
+#pragma unroll
+                for (int j = 0; j < kHalf; ++j) acc[j] = fmaf(s, (float)c[j], acc[j]);
+                if (kMin) {
+                    const float m = fmaf(8.0f, s, __half2float(__ushort_as_half(low.one[gr])));
+                    const float4 *sum = (const float4 *)(xsums + (xs * kGroups + gr) * kN + half * kHalf);
+#pragma unroll
+                    for (int j = 0; j < kHalf; j += 4) {
+                        const float4 v = sum[j / 4];
+                        acc[j] = fmaf(m, v.x, acc[j]);
+                        acc[j + 1] = fmaf(m, v.y, acc[j + 1]);
+                        acc[j + 2] = fmaf(m, v.z, acc[j + 2]);
+                        acc[j + 3] = fmaf(m, v.w, acc[j + 3]);
+                    }
+                }
+            }
+            if (!ok) break;
+            if (kMin) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.x_empty[xs]);
+            }
+            if (splits == 1 && it % per == per - 1) {
+                const int row = (tile0 + it / per * tile_step) * 128 + quad * 32 + lane;
+                if (row < p.rows)
+#pragma unroll
+                    for (int j = 0; j < kHalf; ++j)
+                        if (half * kHalf + j < nx) store_y(p, b0 + half * kHalf + j, row, 0.0625f * acc[j]);
+            }
+        }
+        if (!ok) {
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j) acc[j] = __int_as_float(0x7fc00000);
+            /* loud: every tile of this CTA */
+            if (splits == 1)
+                for (int t = 0; t < my_tiles; ++t) {
+                    const int row = (tile0 + t * tile_step) * 128 + quad * 32 + lane;
+                    if (row < p.rows)
+                        for (int j = 0; j < kHalf; ++j)
+                            if (half * kHalf + j < nx) store_y(p, b0 + half * kHalf + j, row, acc[0]);
+                }
+        }
+    } else if (warp == kTcUnpack + kTcEpi) {
+        /* ---- products ---- */
+        if (lane == 0) {
+            bool ok = true;
+            for (int it = 0, d = 0; it < total && ok; ++it) {
+                const int buf = it & 1, xs = it % kTcXDepth;
+                if (!mbar_wait(&sh.a_full[buf], (it >> 1) & 1, abort_flag) ||
+                    !mbar_wait(&sh.x_full[xs], (it / kTcXDepth) & 1, abort_flag)) {
+                    *abort_flag = 1;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t xt = smem_u32(xring + xs * tc_x_stage(kN));
+#pragma unroll
+                for (int gr = 0; gr < kGroups; ++gr, ++d) {
+                    const int acc_buf = d % kTcD;
+                    if (d >= kTcD && !mbar_wait(&sh.d_empty[acc_buf], ((d / kTcD) & 1) ^ 1, abort_flag)) {
+                        *abort_flag = 1;
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = gr * kPer; k < (gr + 1) * kPer; ++k)
+                        tc_mma_i8_ta(tmem_d + acc_buf * kN, tmem + buf * 64 + k * 8,
+                                     tc_desc(xt + (k / 4) * kN * 128 + (k % 4) * 32), tc_idesc(kN), k != gr * kPer);
+                    tc_commit(&sh.d_full[acc_buf]);
+                }
+                tc_commit(&sh.a_empty[buf]);
+                tc_commit(&sh.x_empty[xs]);
+            }
+            /* every product issued is complete before the tensor memory is freed */
+            tc_commit(&sh.drain);
+            if (!mbar_wait(&sh.drain, 0u, never)) *abort_flag = 1;
+        }
+    } else {
+        /* ---- vectors, and (with minima) their sums ---- */
+        const int lw = warp - kTcUnpack - kTcEpi - 1;
+        const bool x_aligned = (((uintptr_t)p.x | (uintptr_t)p.x_stride) & 15) == 0;
+        /* a loader warp has every kTcLoad-th pair of rows: 16 lanes a row */
+        auto load = [&](int it) -> bool {
+            if (it < total) {
+                const int xs = it % kTcXDepth;
+                if (it >= kTcXDepth && !mbar_wait(&sh.x_empty[xs], ((it / kTcXDepth) & 1) ^ 1, abort_flag)) return false;
+                const int c0 = (st0 + it % per) * kStageBlocks * kQ4Block + (lane & 15) * 16;
+                uint8_t *tile = xring + xs * tc_x_stage(kN) + ((lane & 15) >> 3) * kN * 128;
+                for (int n = lw * 2 + (lane >> 4); n < nx; n += 2 * kTcLoad)
+                    stage_x16(tile + n * 128 + (((lane & 7) ^ (n & 7)) << 4), p.x + (size_t)(b0 + n) * p.x_stride, c0,
+                              p.cols, x_aligned);
+            }
+            cp_async_commit();
+            return true;
+        };
+        bool ok = true;
+        for (int i = 0; i < kTcXDepth - 1; ++i) load(i);
+        for (int it = 0; it < total; ++it) {
+            const int xs = it % kTcXDepth;
+            cp_async_wait<kTcXDepth - 2>();
+            __syncwarp();
+            if (kMin) {
+                /* 16 times the sum of each group of this warp's rows */
+                const uint8_t *st = xring + xs * tc_x_stage(kN);
+                for (int i = lane; i < kN / kTcLoad * kGroups; i += 32) {
+                    const int gr = i % kGroups, pair = i / kGroups;
+                    const int n = (pair >> 1) * 2 * kTcLoad + lw * 2 + (pair & 1);
+                    if (n >= nx) continue;
+                    int sum = 0;
+                    for (int c = gr * kPer * 2; c < (gr + 1) * kPer * 2; ++c) {
+                        const uint4 v = *(const uint4 *)(st + (c >> 3) * kN * 128 + n * 128 + (((c & 7) ^ (n & 7)) << 4));
+                        sum = __dp4a((int)v.x, 0x10101010, __dp4a((int)v.y, 0x10101010, sum));
+                        sum = __dp4a((int)v.z, 0x10101010, __dp4a((int)v.w, 0x10101010, sum));
+                    }
+                    xsums[(xs * kGroups + gr) * kN + n] = (float)sum;
+                }
+            }
+            /* the copies (and stores) become visible to the tensor core */
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.x_full[xs]);
+            ok = load(it + kTcXDepth - 1);
+            if (!__all_sync(0xffffffffu, ok)) {
+                *abort_flag = 1;
+                break;
+            }
+        }
+        cp_async_wait<0>();
+    }
+
+    __syncwarp();
+    if (splits > 1) {
+        /* The CTAs of a tile: each gets every part's sums of kN / splits
+         * streams, [part][stream][128 rows] where the rings were, and adds
+         * them in order. */
+        const int mine = kN / splits;
+        float *parts = (float *)smem;
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (warp >= kTcUnpack && warp < kTcUnpack + kTcEpi) {
+            const int quad = warp & 3, half = (warp - kTcUnpack) >> 2;
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j) {
+                const int n = half * kHalf + j;
+                const uint32_t here = smem_u32(parts + ((size_t)split * mine + n % mine) * 128 + quad * 32 + lane);
+                uint32_t there;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(n / mine));
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(per > 0 ? acc[j] : 0.0f) : "memory");
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        for (int i = threadIdx.x; i < mine * 128; i += 32 * kTcWarps) {
+            const int n = split * mine + (i >> 7), row = tile0 * 128 + (i & 127);
+            if (n >= nx || row >= p.rows) continue;
+            float sum = 0.0f;
+            for (int s = 0; s < splits; ++s) sum += parts[((size_t)s * mine + (i >> 7)) * 128 + (i & 127)];
+            store_y(p, b0 + n, row, 0.0625f * sum);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kTcUnpack + kTcEpi) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols) : "memory");
+    }
+}
+
+template <int kN, int kGroup, bool kMin>
+cudaError_t launch_tc(const MatvecParams &p, int x_base, int chunks, int num_sms, cudaStream_t st) {
+    const int tiles = (p.rows + 127) / 128, stages = (q4_blocks(p.cols) + kStageBlocks - 1) / kStageBlocks;
+    /* CTAs of a tile: as many as leave each an SM and two stages */
+    int splits = 1;
+    while (splits < kTcMaxSplit && (long long)tiles * chunks * splits * 2 <= num_sms && splits * 4 <= stages) splits *= 2;
+    const void *fn = (const void *)q4_tc_kernel<kN, kGroup, kMin>;
+    constexpr int smem = tc_smem<kN, kGroup, kMin>();
+    cudaError_t e = raise_smem(fn, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(splits > 1 ? tiles * splits : std::min(tiles, num_sms)), (unsigned)chunks);
+    cfg.blockDim = dim3(32 * kTcWarps);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, q4_tc_kernel<kN, kGroup, kMin>, p, splits, x_base);
+}
+
+template <int kGroup, bool kMin>
+cudaError_t launch_tc_all(const MatvecParams &p, int num_sms, cudaStream_t st) {
+    /* whole chunks of 64 streams, then the smallest tile that has the rest */
+    const int whole = p.streams / 64, rest = p.streams % 64;
+    if (whole > 0) {
+        const cudaError_t e = launch_tc<64, kGroup, kMin>(p, 0, whole, num_sms, st);
+        if (e != cudaSuccess || rest == 0) return e;
+    }
+    return rest <= 16   ? launch_tc<16, kGroup, kMin>(p, whole * 64, 1, num_sms, st)
+           : rest <= 32 ? launch_tc<32, kGroup, kMin>(p, whole * 64, 1, num_sms, st)
+                        : launch_tc<64, kGroup, kMin>(p, whole * 64, 1, num_sms, st);
+}
+
 template <int kGroup, bool kMin> cudaError_t launch_matvec(const MatvecParams &p, int num_sms, cudaStream_t st) {
+    if (p.streams > kMmaStreams) return launch_tc_all<kGroup, kMin>(p, num_sms, st);
     return p.streams <= 3 ? launch_mma<kGroup, kMin, 4>(p, num_sms, st) : launch_mma<kGroup, kMin, 3>(p, num_sms, st);
 }
 
@@ -717,6 +1139,9 @@ int convert_q4(const char *op, const lal_tail_q4 *w, void *d_w, int64_t w_stride
 }
 
 }  // namespace
+}  // namespace lal
+
+using namespace lal;
 
 extern "C" {
 
