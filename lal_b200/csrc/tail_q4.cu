@@ -653,12 +653,14 @@ cudaError_t launch_mma(const MatvecParams &p, int num_sms, cudaStream_t st) {
  * memory.
  *
  * Every wait is bounded; one that runs out makes the tile's results NaN. */
-constexpr int kTcUnpack = 4, kTcEpi = 8, kTcLoad = 2;
-constexpr int kTcWarps = kTcUnpack + kTcEpi + 1 + kTcLoad;
+constexpr int kTcUnpack = 8, kTcEpi = 16, kTcLoad = 4;
+constexpr int kTcIssue = kTcUnpack + kTcEpi; /* the warp that issues the products */
+constexpr int kTcWarps = kTcIssue + 1 + kTcLoad;
 constexpr int kTcD = 4;        /* accumulators */
 constexpr int kTcWDepth = 6;   /* stages of a warp's weight ring */
 constexpr int kTcXDepth = 4;   /* stages of the vectors */
-constexpr int kTcWStage = 32 * kStageBlocks * 16;
+constexpr int kTcHalf = kStageBlocks / 2;         /* blocks of a stage that an unpacking warp has */
+constexpr int kTcWStage = 32 * kTcHalf * 16;
 constexpr int kTcMaxSplit = 8;
 
 struct TcShared {
@@ -679,18 +681,18 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-/* D[tensor memory] (+)= A[tensor memory] * B[shared memory]^T, int8 x int8 -> int32 */
-__device__ __forceinline__ void tc_mma_i8_ta(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\t"
-                 "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
-                 "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate), "r"(0));
-}
 /* Shared-memory descriptor of rows of 128 bytes with the 128-byte swizzle
- * (8-row groups 1024 bytes apart); 32 bytes further is the next K step. */
-__device__ __forceinline__ uint64_t tc_desc(uint32_t at) {
-    return (uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1 << 46 |
-           (uint64_t)2 << 61;
+ * (8-row groups 1024 bytes apart): its low word from the address in units of
+ * 16 bytes, to which a K step of 32 bytes adds 2, and its high word. */
+constexpr uint32_t kTcDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t tc_desc_low(uint32_t at) { return ((at >> 4) & 0x3FFFu) | 1u << 16; }
+/* D[tensor memory] (+)= A[tensor memory] * B[shared memory]^T, int8 x int8 -> int32 */
+__device__ __forceinline__ void tc_mma_i8_ta(uint32_t d, uint32_t a, uint32_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "mov.b64 b, {%2, %6};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], b, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+                 "r"(a), "r"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(kTcDescHigh));
 }
 /* int32 accumulators, signed int8 operands, both K-major, 128 rows by n */
 __device__ constexpr uint32_t tc_idesc(int n) {
@@ -701,10 +703,59 @@ __device__ __forceinline__ void tc_store8(uint32_t at, const uint32_t (&r)[8]) {
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
-__device__ __forceinline__ void tc_load8(uint32_t at, int *r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(at));
+template <int kCount> __device__ __forceinline__ void tc_load(uint32_t at, int (&r)[kCount]) {
+    if constexpr (kCount == 16)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                     "%14, %15}, [%16];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                       "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                     : "r"(at));
+    else if constexpr (kCount == 8)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                     : "r"(at));
+    else
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(at));
+    /* the wait names the registers, so that nothing reads them before it */
+    if constexpr (kCount == 16)
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                       "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                     :
+                     : "memory");
+    else if constexpr (kCount == 8)
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+                     :
+                     : "memory");
+    else
+        asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]) : : "memory");
+}
+
+/* The stages of a CTA in order: every tile's range of K. */
+struct TcWalk {
+    int tile, st, n = 0;
+    __device__ TcWalk(int tile0, int st0) : tile(tile0), st(st0) {}
+    __device__ void next(int st0, int st1, int tile_step) {
+        ++n;
+        if (++st == st1) st = st0, tile += tile_step;
+    }
+};
+
+/* A bounded wait, as mbar_wait, that reads a clock only once it has waited long. */
+__device__ __forceinline__ bool tc_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag) {
+    constexpr long long kClocks = 4000000000LL; /* about two seconds */
+    long long t0 = 0;
+    for (uint32_t it = 1; !mbar_try(b, parity); ++it) {
+        if ((it & 255u) != 0) continue;
+        if (*abort_flag) return false;
+        const long long now = clock64();
+        if (t0 == 0) t0 = now;
+        if (now - t0 > kClocks) return false;
+    }
+    return true;
 }
 
 template <int kN, int kGroup, bool kMin>
@@ -712,7 +763,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
     extern __shared__ uint8_t smem_raw[];
     __shared__ TcShared sh;
     constexpr int kPer = kGroup / kQ4Block, kGroups = kStageBlocks / kPer; /* blocks a group, groups a stage */
-    constexpr int kHalf = kN / 2;                                          /* streams of an epilogue warp */
+    constexpr int kMine = kN / (kTcEpi / 4);                               /* streams of an epilogue warp */
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t *xring = smem;                                      /* kTcXDepth stages of two swizzled tiles */
     uint8_t *wring = xring + kTcXDepth * tc_x_stage(kN);        /* of each unpacking warp */
@@ -739,7 +790,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
         mbar_fence_init();
     }
     constexpr int kCols = 128 + kTcD * kN <= 256 ? 256 : 512;
-    if (warp == kTcUnpack + kTcEpi) {
+    if (warp == kTcIssue) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(kCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -749,50 +800,64 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
     tc_fence_after();
     const uint32_t tmem = sh.tmem, tmem_d = tmem + 128; /* two A operands of 64 columns, then the accumulators */
 
-    float acc[kHalf]; /* of an epilogue thread */
+    float acc[kMine]; /* of an epilogue thread */
 
     if (warp < kTcUnpack) {
-        /* ---- weights: 4 bits in global memory -> int8 in tensor memory ---- */
+        /* ---- weights: 4 bits in global memory -> int8 in tensor memory;
+         * rows of one quarter of tensor memory, half of a stage's blocks ---- */
         uint8_t *ring = wring + warp * kTcWDepth * kTcWStage;
-        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-        auto load = [&](int it) {
-            if (it < total) {
-                const int row0 = (tile0 + it / per * tile_step) * 128 + warp * 32, k0 = (st0 + it % per) * kStageBlocks;
-                const bool in = k0 + (lane & 7) < nb;
-                const uint32_t dst = smem_u32(ring + it % kTcWDepth * kTcWStage) + (lane >> 3) * 128;
+        const int quad = warp & 3, half = warp >> 2;
+        const uint32_t to = tmem + ((uint32_t)(quad * 32) << 16) + half * (kTcHalf * 8);
+        const int k = half * kTcHalf + (lane & 3); /* this lane's block of a stage, of rows lane / 4, + 8, ... */
+        const uint32_t dst = smem_u32(ring) + lane * 16; /* 4 blocks a row; swizzled by the row's pair */
+        TcWalk ahead(tile0, st0);
+        auto load = [&](int slot) {
+            if (ahead.n < total) {
+                const int row0 = ahead.tile * 128 + quad * 32 + (lane >> 2), kb = ahead.st * kStageBlocks + k;
+                const uint32_t to_slot = (dst + slot * kTcWStage) ^ (((lane >> 3) & 3) << 4);
+                if (row0 + 24 < p.rows && kb < nb) {
+                    const uint8_t *src = p.q + ((size_t)row0 * nb + kb) * 16;
+                    const size_t step = (size_t)nb * 128; /* 8 rows */
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int r = (lane >> 3) + 4 * j;
-                    const uint8_t *src = p.q + ((size_t)min(row0 + r, p.rows - 1) * nb + (in ? k0 + (lane & 7) : 0)) * 16;
-                    cp_async16(dst + j * 512 + (((lane & 7) ^ (r & 7)) << 4), src, in ? 16 : 0);
+                    for (int j = 0; j < 4; ++j) cp_async16(to_slot + j * 512, src + j * step, 16);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        cp_async16(to_slot + j * 512, p.q + ((size_t)min(row0 + 8 * j, p.rows - 1) * nb + min(kb, nb - 1)) * 16,
+                                   kb < nb ? 16 : 0);
                 }
             }
+            ahead.next(st0, st1, tile_step);
             cp_async_commit();
         };
         for (int i = 0; i < kTcWDepth - 1; ++i) load(i);
+        int slot = 0;
         for (int it = 0; it < total; ++it) {
             cp_async_wait<kTcWDepth - 2>();
             __syncwarp();
-            load(it + kTcWDepth - 1);
+            load(slot == 0 ? kTcWDepth - 1 : slot - 1);
+            uint4 v[kTcHalf];
+            const uint8_t *row = ring + slot * kTcWStage + lane * 64;
+#pragma unroll
+            for (int i = 0; i < kTcHalf; ++i) v[i] = *(const uint4 *)(row + ((i ^ ((lane >> 1) & 3)) << 4));
+            slot = slot + 1 == kTcWDepth ? 0 : slot + 1;
             const int buf = it & 1;
-            if (it >= 2 && !mbar_wait(&sh.a_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag)) {
+            if (it >= 2 && !tc_wait(&sh.a_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag)) {
                 *abort_flag = 1;
                 break;
             }
             __syncwarp();
             tc_fence_after();
-            const uint8_t *row = ring + it % kTcWDepth * kTcWStage + lane * 128;
 #pragma unroll
-            for (int k = 0; k < kStageBlocks; ++k) {
-                const uint4 v = *(const uint4 *)(row + ((k ^ (lane & 7)) << 4));
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            for (int i = 0; i < kTcHalf; ++i) {
+                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
                 uint32_t o[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    o[i] = ((w[i] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
-                    o[4 + i] = (w[i] & 0xf0f0f0f0u) ^ 0x80808080u;
+                for (int j = 0; j < 4; ++j) {
+                    o[j] = ((w[j] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+                    o[4 + j] = (w[j] & 0xf0f0f0f0u) ^ 0x80808080u;
                 }
-                tc_store8(lanes + buf * 64 + k * 8, o);
+                tc_store8(to + buf * 64 + i * 8, o);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
@@ -800,10 +865,10 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             if (lane == 0) mbar_arrive(&sh.a_full[buf]);
         }
         cp_async_wait<0>();
-    } else if (warp < kTcUnpack + kTcEpi) {
+    } else if (warp < kTcIssue) {
         /* ---- accumulators: scaled and added ---- */
-        const int quad = warp & 3, half = (warp - kTcUnpack) >> 2;
-        const uint32_t lanes = tmem_d + ((uint32_t)(quad * 32) << 16) + half * kHalf;
+        const int quad = warp & 3, part = (warp - kTcUnpack) >> 2;
+        const uint32_t lanes = tmem_d + ((uint32_t)(quad * 32) << 16) + part * kMine;
         /* a row's scales (and minima) of a stage, one load where all rows' are aligned to it */
         using Pack = std::conditional_t<kGroups == 8, uint4, std::conditional_t<kGroups == 4, uint2, uint32_t>>;
         union Row {
@@ -813,57 +878,58 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
         } scale, low, scale_next, low_next;
         const bool s_aligned =
             (((uintptr_t)p.scale | (kMin ? (uintptr_t)p.min : 0) | (uintptr_t)(groups * 2)) & (2 * kGroups - 1)) == 0;
-        auto load_scales = [&](int it) {
-            const int row = min((tile0 + it / per * tile_step) * 128 + quad * 32 + lane, p.rows - 1);
-            const int g0 = (st0 + it % per) * kGroups;
-            const size_t at = (size_t)row * groups + g0;
-            if (s_aligned && g0 + kGroups <= groups) {
-                scale_next.all = __ldg((const Pack *)(p.scale + at));
-                if (kMin) low_next.all = __ldg((const Pack *)(p.min + at));
-            } else {
+        TcWalk ahead(tile0, st0);
+        auto load_scales = [&] {
+            if (ahead.n < total) {
+                const int row = min(ahead.tile * 128 + quad * 32 + lane, p.rows - 1), g0 = ahead.st * kGroups;
+                const size_t at = (size_t)row * groups + g0;
+                if (s_aligned && g0 + kGroups <= groups) {
+                    scale_next.all = __ldg((const Pack *)(p.scale + at));
+                    if (kMin) low_next.all = __ldg((const Pack *)(p.min + at));
+                } else {
 #pragma unroll
-                for (int i = 0; i < kGroups; ++i) {
-                    scale_next.one[i] = g0 + i < groups ? __ldg((const unsigned short *)p.scale + at + i) : 0;
-                    if (kMin) low_next.one[i] = g0 + i < groups ? __ldg((const unsigned short *)p.min + at + i) : 0;
+                    for (int i = 0; i < kGroups; ++i) {
+                        scale_next.one[i] = g0 + i < groups ? __ldg((const unsigned short *)p.scale + at + i) : 0;
+                        if (kMin) low_next.one[i] = g0 + i < groups ? __ldg((const unsigned short *)p.min + at + i) : 0;
+                    }
                 }
             }
+            ahead.next(st0, st1, tile_step);
         };
-        if (total > 0) load_scales(0);
+        load_scales();
         bool ok = true;
-        for (int it = 0, d = 0; it < total; ++it) {
-            if (it % per == 0)
+        TcWalk at(tile0, st0);
+        for (int d = 0, xs = 0, xs_round = 0; at.n < total; at.next(st0, st1, tile_step)) {
+            if (at.st == st0)
 #pragma unroll
-                for (int j = 0; j < kHalf; ++j) acc[j] = 0.0f;
+                for (int j = 0; j < kMine; ++j) acc[j] = 0.0f;
             scale.all = scale_next.all;
             if (kMin) low.all = low_next.all;
-            if (it + 1 < total) load_scales(it + 1);
-            const int xs = it % kTcXDepth;
-            if (kMin && ok && !mbar_wait(&sh.x_full[xs], (it / kTcXDepth) & 1, abort_flag)) ok = false;
+            load_scales();
+            if (kMin && !tc_wait(&sh.x_full[xs], xs_round & 1, abort_flag)) ok = false;
 #pragma unroll
             for (int gr = 0; gr < kGroups; ++gr, ++d) {
                 const int buf = d % kTcD;
-                if (ok && !mbar_wait(&sh.d_full[buf], (d / kTcD) & 1, abort_flag)) ok = false;
+                if (ok && !tc_wait(&sh.d_full[buf], (d / kTcD) & 1, abort_flag)) ok = false;
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     *abort_flag = 1;
                     break;
                 }
                 tc_fence_after();
-                int c[kHalf];
-#pragma unroll
-                for (int j = 0; j < kHalf; j += 8) tc_load8(lanes + buf * kN + j, c + j);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                int c[kMine];
+                tc_load<kMine>(lanes + buf * kN, c);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.d_empty[buf]);
                 const float s = __half2float(__ushort_as_half(scale.one[gr]));
 #pragma unroll
-                for (int j = 0; j < kHalf; ++j) acc[j] = fmaf(s, (float)c[j], acc[j]);
+                for (int j = 0; j < kMine; ++j) acc[j] = fmaf(s, (float)c[j], acc[j]);
                 if (kMin) {
                     const float m = fmaf(8.0f, s, __half2float(__ushort_as_half(low.one[gr])));
-                    const float4 *sum = (const float4 *)(xsums + (xs * kGroups + gr) * kN + half * kHalf);
+                    const float4 *sum = (const float4 *)(xsums + (xs * kGroups + gr) * kN + part * kMine);
 #pragma unroll
-                    for (int j = 0; j < kHalf; j += 4) {
+                    for (int j = 0; j < kMine; j += 4) {
                         const float4 v = sum[j / 4];
                         acc[j] = fmaf(m, v.x, acc[j]);
                         acc[j + 1] = fmaf(m, v.y, acc[j + 1]);
@@ -876,44 +942,47 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             if (kMin) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.x_empty[xs]);
+                if (++xs == kTcXDepth) xs = 0, ++xs_round;
             }
-            if (splits == 1 && it % per == per - 1) {
-                const int row = (tile0 + it / per * tile_step) * 128 + quad * 32 + lane;
+            if (splits == 1 && at.st == st1 - 1) {
+                const int row = at.tile * 128 + quad * 32 + lane;
                 if (row < p.rows)
 #pragma unroll
-                    for (int j = 0; j < kHalf; ++j)
-                        if (half * kHalf + j < nx) store_y(p, b0 + half * kHalf + j, row, 0.0625f * acc[j]);
+                    for (int j = 0; j < kMine; ++j)
+                        if (part * kMine + j < nx) store_y(p, b0 + part * kMine + j, row, 0.0625f * acc[j]);
             }
         }
         if (!ok) {
 #pragma unroll
-            for (int j = 0; j < kHalf; ++j) acc[j] = __int_as_float(0x7fc00000);
+            for (int j = 0; j < kMine; ++j) acc[j] = __int_as_float(0x7fc00000);
             /* loud: every tile of this CTA */
             if (splits == 1)
                 for (int t = 0; t < my_tiles; ++t) {
                     const int row = (tile0 + t * tile_step) * 128 + quad * 32 + lane;
                     if (row < p.rows)
-                        for (int j = 0; j < kHalf; ++j)
-                            if (half * kHalf + j < nx) store_y(p, b0 + half * kHalf + j, row, acc[0]);
+                        for (int j = 0; j < kMine; ++j)
+                            if (part * kMine + j < nx) store_y(p, b0 + part * kMine + j, row, acc[0]);
                 }
         }
-    } else if (warp == kTcUnpack + kTcEpi) {
+    } else if (warp == kTcIssue) {
         /* ---- products ---- */
         if (lane == 0) {
             bool ok = true;
+            const uint32_t x0 = tc_desc_low(smem_u32(xring));
+            int xs = 0, xs_round = 0;
             for (int it = 0, d = 0; it < total && ok; ++it) {
-                const int buf = it & 1, xs = it % kTcXDepth;
-                if (!mbar_wait(&sh.a_full[buf], (it >> 1) & 1, abort_flag) ||
-                    !mbar_wait(&sh.x_full[xs], (it / kTcXDepth) & 1, abort_flag)) {
+                const int buf = it & 1;
+                if (!tc_wait(&sh.x_full[xs], xs_round & 1, abort_flag) ||
+                    !tc_wait(&sh.a_full[buf], (it >> 1) & 1, abort_flag)) {
                     *abort_flag = 1;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t xt = smem_u32(xring + xs * tc_x_stage(kN));
+                const uint32_t xt = x0 + xs * (tc_x_stage(kN) >> 4);
 #pragma unroll
                 for (int gr = 0; gr < kGroups; ++gr, ++d) {
                     const int acc_buf = d % kTcD;
-                    if (d >= kTcD && !mbar_wait(&sh.d_empty[acc_buf], ((d / kTcD) & 1) ^ 1, abort_flag)) {
+                    if (d >= kTcD && !tc_wait(&sh.d_empty[acc_buf], ((d / kTcD) & 1) ^ 1, abort_flag)) {
                         *abort_flag = 1;
                         ok = false;
                         break;
@@ -921,39 +990,48 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                     tc_fence_after();
 #pragma unroll
                     for (int k = gr * kPer; k < (gr + 1) * kPer; ++k)
-                        tc_mma_i8_ta(tmem_d + acc_buf * kN, tmem + buf * 64 + k * 8,
-                                     tc_desc(xt + (k / 4) * kN * 128 + (k % 4) * 32), tc_idesc(kN), k != gr * kPer);
+                        tc_mma_i8_ta(tmem_d + acc_buf * kN, tmem + buf * 64 + k * 8, xt + (k / 4) * (kN * 128 >> 4) + (k % 4) * 2,
+                                     tc_idesc(kN), k != gr * kPer);
                     tc_commit(&sh.d_full[acc_buf]);
                 }
                 tc_commit(&sh.a_empty[buf]);
                 tc_commit(&sh.x_empty[xs]);
+                if (++xs == kTcXDepth) xs = 0, ++xs_round;
             }
             /* every product issued is complete before the tensor memory is freed */
             tc_commit(&sh.drain);
-            if (!mbar_wait(&sh.drain, 0u, never)) *abort_flag = 1;
+            if (!tc_wait(&sh.drain, 0u, never)) *abort_flag = 1;
         }
     } else {
         /* ---- vectors, and (with minima) their sums ---- */
-        const int lw = warp - kTcUnpack - kTcEpi - 1;
+        const int lw = warp - kTcIssue - 1;
         const bool x_aligned = (((uintptr_t)p.x | (uintptr_t)p.x_stride) & 15) == 0;
         /* a loader warp has every kTcLoad-th pair of rows: 16 lanes a row */
-        auto load = [&](int it) -> bool {
-            if (it < total) {
-                const int xs = it % kTcXDepth;
-                if (it >= kTcXDepth && !mbar_wait(&sh.x_empty[xs], ((it / kTcXDepth) & 1) ^ 1, abort_flag)) return false;
-                const int c0 = (st0 + it % per) * kStageBlocks * kQ4Block + (lane & 15) * 16;
-                uint8_t *tile = xring + xs * tc_x_stage(kN) + ((lane & 15) >> 3) * kN * 128;
-                for (int n = lw * 2 + (lane >> 4); n < nx; n += 2 * kTcLoad)
-                    stage_x16(tile + n * 128 + (((lane & 7) ^ (n & 7)) << 4), p.x + (size_t)(b0 + n) * p.x_stride, c0,
-                              p.cols, x_aligned);
+        const int n0 = lw * 2 + (lane >> 4);
+        const int8_t *x0 = p.x + (size_t)(b0 + min(n0, nx - 1)) * p.x_stride;
+        const size_t x_step = (size_t)(2 * kTcLoad) * p.x_stride;
+        const uint32_t d0 = ((lane & 15) >> 3) * kN * 128 + n0 * 128 + (((lane & 7) ^ (n0 & 7)) << 4);
+        static_assert(2 * kTcLoad == 8, "a lane's rows are 8 apart: the same place in the swizzle");
+        TcWalk ahead(tile0, st0);
+        auto load = [&](int xs, int round) -> bool {
+            if (ahead.n < total) {
+                if (round > 0 && !tc_wait(&sh.x_empty[xs], (round & 1) ^ 1, abort_flag)) return false;
+                const int c0 = ahead.st * kStageBlocks * kQ4Block + (lane & 15) * 16;
+                uint8_t *dst = xring + xs * tc_x_stage(kN) + d0;
+                const int8_t *x = x0;
+                if (x_aligned && c0 + 16 <= p.cols) {
+                    x += c0;
+                    for (int n = n0; n < nx; n += 2 * kTcLoad, x += x_step, dst += 1024) cp_async16_l1(smem_u32(dst), x, 16);
+                } else {
+                    for (int n = n0; n < nx; n += 2 * kTcLoad, x += x_step, dst += 1024) stage_x16(dst, x, c0, p.cols, x_aligned);
+                }
             }
+            ahead.next(st0, st1, tile_step);
             cp_async_commit();
             return true;
         };
-        bool ok = true;
-        for (int i = 0; i < kTcXDepth - 1; ++i) load(i);
-        for (int it = 0; it < total; ++it) {
-            const int xs = it % kTcXDepth;
+        for (int i = 0; i < kTcXDepth - 1; ++i) load(i, 0);
+        for (int it = 0, xs = 0, xl = kTcXDepth - 1, round = 0; it < total; ++it) {
             cp_async_wait<kTcXDepth - 2>();
             __syncwarp();
             if (kMin) {
@@ -964,7 +1042,9 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                     const int n = (pair >> 1) * 2 * kTcLoad + lw * 2 + (pair & 1);
                     if (n >= nx) continue;
                     int sum = 0;
-                    for (int c = gr * kPer * 2; c < (gr + 1) * kPer * 2; ++c) {
+#pragma unroll
+                    for (int j = 0; j < kPer * 2; ++j) {
+                        const int c = gr * kPer * 2 + j;
                         const uint4 v = *(const uint4 *)(st + (c >> 3) * kN * 128 + n * 128 + (((c & 7) ^ (n & 7)) << 4));
                         sum = __dp4a((int)v.x, 0x10101010, __dp4a((int)v.y, 0x10101010, sum));
                         sum = __dp4a((int)v.z, 0x10101010, __dp4a((int)v.w, 0x10101010, sum));
@@ -976,7 +1056,9 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.x_full[xs]);
-            ok = load(it + kTcXDepth - 1);
+            const bool ok = load(xl, round);
+            if (++xs == kTcXDepth) xs = 0;
+            if (++xl == kTcXDepth) xl = 0, ++round;
             if (!__all_sync(0xffffffffu, ok)) {
                 *abort_flag = 1;
                 break;
@@ -994,11 +1076,11 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
         float *parts = (float *)smem;
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (warp >= kTcUnpack && warp < kTcUnpack + kTcEpi) {
-            const int quad = warp & 3, half = (warp - kTcUnpack) >> 2;
+        if (warp >= kTcUnpack && warp < kTcIssue) {
+            const int quad = warp & 3, part = (warp - kTcUnpack) >> 2;
 #pragma unroll
-            for (int j = 0; j < kHalf; ++j) {
-                const int n = half * kHalf + j;
+            for (int j = 0; j < kMine; ++j) {
+                const int n = part * kMine + j;
                 const uint32_t here = smem_u32(parts + ((size_t)split * mine + n % mine) * 128 + quad * 32 + lane);
                 uint32_t there;
                 asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(n / mine));
@@ -1017,7 +1099,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kTcUnpack + kTcEpi) {
+    if (warp == kTcIssue) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols) : "memory");
     }
