@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 using namespace lal;
 
@@ -49,76 +50,85 @@ constexpr float kFltMax = 3.4028234663852886e38f;
  * is computed in 64 bits, clear of overflow and of denormal rounding */
 constexpr float kWideHi = 1e37f, kWideLo = 1e-30f;
 
-/* Eight elements of a row from p on, of which `n` exist, as wide as p's
- * alignment allows (rows of 16-bit elements may begin at any even address). */
-template <typename T> __device__ __forceinline__ void get8(const T *p, int n, float (&v)[8]) {
-    if (n < 8) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
-        return;
-    }
+/* Eight elements of a row as they lie in memory. */
+template <typename T> union Eight {
+    uint4 q[sizeof(T) / 2];
+    uint32_t w[2 * sizeof(T)];
+    unsigned short s[4 * sizeof(T)];
+    T e[8];
+    __device__ Eight() {}
+};
+
+/* From p on, of which `n` exist (the others 0).  kWide: all do, at a 16-byte
+ * boundary; else as wide as p's alignment allows (rows of 16-bit elements may
+ * begin at any even address). */
+template <bool kWide, typename T> __device__ __forceinline__ void get8(const T *p, int n, Eight<T> &v) {
     const unsigned at = (unsigned)(uintptr_t)p;
-    union Raw {
-        uint4 q[sizeof(T) / 2];
-        uint32_t w[2 * sizeof(T)];
-        T e[8];
-        __device__ Raw() {}
-    } raw;
-    if ((at & 15) == 0) {
+    if (kWide || (n == 8 && (at & 15) == 0)) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw.q[i] = ((const uint4 *)p)[i];
-    } else if (sizeof(T) == 4 || (at & 3) == 0) {
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v.q[i] = ((const uint4 *)p)[i];
+    } else if (n == 8 && (sizeof(T) == 4 || (at & 3) == 0)) {
 #pragma unroll
-        for (int i = 0; i < 2 * (int)sizeof(T); ++i) raw.w[i] = ((const uint32_t *)p)[i];
-    } else {
-        raw.e[0] = p[0];
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) v.w[i] = ((const uint32_t *)p)[i];
+    } else if (n == 8) {
         const uint32_t *w = (const uint32_t *)(p + 1);
         const uint32_t m0 = w[0], m1 = w[1], m2 = w[2];
-        const unsigned short last = ((const unsigned short *)p)[7];
-        const uint32_t first = *(const unsigned short *)&raw.e[0];
-        raw.w[0] = first | m0 << 16;
-        raw.w[1] = __funnelshift_r(m0, m1, 16);
-        raw.w[2] = __funnelshift_r(m1, m2, 16);
-        raw.w[3] = m2 >> 16 | (uint32_t)last << 16;
-    }
+        const uint32_t first = ((const unsigned short *)p)[0], last = ((const unsigned short *)p)[7];
+        v.w[0] = first | m0 << 16;
+        v.w[1] = __funnelshift_r(m0, m1, 16);
+        v.w[2] = __funnelshift_r(m1, m2, 16);
+        v.w[3] = m2 >> 16 | last << 16;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32(raw.e[i]);
+        for (int i = 0; i < 8; ++i) v.e[i] = i < n ? p[i] : from_f32<T>(0.0f);
+    }
 }
-
-template <typename T> __device__ __forceinline__ void put8(T *p, int n, const float (&v)[8]) {
-    if (n < 8) {
+template <bool kWide, typename T> __device__ __forceinline__ void put8(T *p, int n, const Eight<T> &v) {
+    const unsigned at = (unsigned)(uintptr_t)p;
+    if (kWide || (n == 8 && (at & 15) == 0)) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((uint4 *)p)[i] = v.q[i];
+    } else if (n == 8 && (sizeof(T) == 4 || (at & 3) == 0)) {
+#pragma unroll
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) ((uint32_t *)p)[i] = v.w[i];
+    } else if (n == 8) {
+        p[0] = v.e[0];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) ((uint32_t *)(p + 1))[i] = __funnelshift_r(v.w[i], v.w[i + 1], 16);
+        p[7] = v.e[7];
+    } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = from_f32<T>(v[i]);
-        return;
+            if (i < n) p[i] = v.e[i];
     }
-    const unsigned at = (unsigned)(uintptr_t)p;
-    union Raw {
-        uint4 q[sizeof(T) / 2];
-        uint32_t w[2 * sizeof(T)];
-        T e[8];
-        __device__ Raw() {}
-    } raw;
+}
+template <typename T> __device__ __forceinline__ void to8(const Eight<T> &v, float (&f)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw.e[i] = from_f32<T>(v[i]);
-    if ((at & 15) == 0) {
+    for (int i = 0; i < 8; ++i) f[i] = to_f32(v.e[i]);
+}
+/* a + b, rounded to the type.  (16-bit sums rounded once are those rounded to
+ * fp32 first: where fp32 rounds, the smaller term is below 2^-13 of the larger
+ * and the sum far from halfway between two 16-bit numbers.) */
+__device__ __forceinline__ void add8(Eight<float> &a, const Eight<float> &b) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((uint4 *)p)[i] = raw.q[i];
-    } else if (sizeof(T) == 4 || (at & 3) == 0) {
+    for (int i = 0; i < 8; ++i) a.e[i] = __fadd_rn(a.e[i], b.e[i]);
+}
+template <typename T> __device__ __forceinline__ void add8(Eight<T> &a, const Eight<T> &b) {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
 #pragma unroll
-        for (int i = 0; i < 2 * (int)sizeof(T); ++i) ((uint32_t *)p)[i] = raw.w[i];
-    } else {
-        p[0] = raw.e[0];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) ((uint32_t *)(p + 1))[i] = __funnelshift_r(raw.w[i], raw.w[i + 1], 16);
-        p[7] = raw.e[7];
+    for (int i = 0; i < 4; ++i) {
+        T2 u, v;
+        memcpy(&u, &a.w[i], 4);
+        memcpy(&v, &b.w[i], 4);
+        u = __hadd2_rn(u, v);
+        memcpy(&a.w[i], &u, 4);
     }
 }
 
 /* n of eight bytes */
-__device__ __forceinline__ void put_q8(int8_t *p, int n, const uint32_t (&w)[2]) {
+template <bool kWide> __device__ __forceinline__ void put_q8(int8_t *p, int n, const uint32_t (&w)[2]) {
     const unsigned at = (unsigned)(uintptr_t)p;
-    if (n == 8 && (at & 7) == 0) {
+    if (kWide || (n == 8 && (at & 7) == 0)) {
         *(uint2 *)p = make_uint2(w[0], w[1]);
     } else if (n == 8 && (at & 3) == 0) {
         ((uint32_t *)p)[0] = w[0];
@@ -132,13 +142,15 @@ __device__ __forceinline__ void put_q8(int8_t *p, int n, const uint32_t (&w)[2])
 
 /* What the two kinds of rows have of their own: v of eight elements in 32
  * bits, v of one in 64. */
-template <typename T> struct NormRow {
+template <typename T, bool kWide_> struct NormRow {
+    static constexpr bool kWide = kWide_;
     const T *x, *r;
     T *h;
     const float *w;
     int n;
     /* v: 2^-24; 127 / max|v|: 2 * 2^-24; their product: 2^-24; times 127: below 3.1e-5 */
     static constexpr float kBorder = 4e-5f;
+    static constexpr float kRelative = 0.0f;
     static constexpr bool kNorm = true;
     __device__ NormRow(const RowParams &p, int at)
         : x((const T *)p.a + (size_t)at * p.a_stride),
@@ -147,54 +159,80 @@ template <typename T> struct NormRow {
     /* adds the residual, stores the sum, adds its squares to `sum` */
     __device__ void load(int i, float (&v)[8], double &sum) const {
         const int m = min(8, n - i);
-        get8(x + i, m, v);
-        float u[8];
+        Eight<T> a;
+        get8<kWide>(x + i, m, a);
+        Eight<float> u;
+        get8<kWide>(w + i, m, u);
         if (r != nullptr) {
-            get8(r + i, m, u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = to_f32(from_f32<T>(__fadd_rn(v[j], u[j])));
+            Eight<T> b;
+            get8<kWide>(r + i, m, b);
+            add8(a, b);
         }
-        if (h != nullptr) put8(h + i, m, v);
-        get8(w + i, m, u);
+        if (h != nullptr) put8<kWide>(h + i, m, a);
+        to8(a, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             sum = fma((double)v[j], (double)v[j], sum);
-            v[j] = __fmul_rn(v[j], u[j]);
+            v[j] = __fmul_rn(v[j], u.e[j]);
         }
     }
     /* the same v again, by the thread that loaded it */
     __device__ void again(int i, float (&v)[8]) const {
         const int m = min(8, n - i);
-        float u[8];
-        get8(h != nullptr ? (const T *)h + i : x + i, m, v);
-        get8(w + i, m, u);
+        Eight<T> a;
+        get8<kWide>(h != nullptr ? (const T *)h + i : x + i, m, a);
+        Eight<float> u;
+        get8<kWide>(w + i, m, u);
+        to8(a, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], u[j]);
+        for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], u.e[j]);
     }
     __device__ double v64(int i) const { return (double)to_f32(h != nullptr ? h[i] : x[i]) * (double)w[i]; }
 };
 
-template <typename T> struct SwigluRow {
+template <typename T, bool kWide_> struct SwigluRow {
+    static constexpr bool kWide = kWide_;
     const T *g, *u;
     int n;
-    /* expf 2 ulp, 1 + e 0.5, __fdividef 2, the product 0.5 (5 * 2^-23), 127 / max|v| and the
-     * product with it 3 * 2^-24; times 127: below 1e-4 */
-    static constexpr float kBorder = 1.2e-4f;
+    /* Relative errors: exp(-gate) 2^-22 of ex2 and 2^-23 around it, 1 + e 2^-24, its reciprocal 2^-23,
+     * two products 2^-24 each, 127 / max|v| 2^-23, the product with it 2^-24: below 1e-6 */
+    static constexpr float kRelative = 1.2e-6f;
+    static constexpr float kBorder = 0.0f;
     static constexpr bool kNorm = false;
     __device__ SwigluRow(const RowParams &p, int at)
         : g((const T *)p.a + (size_t)at * p.a_stride), u((const T *)p.b + (size_t)at * p.b_stride),
           n(p.n) {}
     __device__ void load(int i, float (&v)[8], double &) const {
         const int m = min(8, n - i);
-        float up[8];
-        get8(g + i, m, v);
-        get8(u + i, m, up);
+        float up[8], low = 0.0f;
+        Eight<T> a, b;
+        get8<kWide>(g + i, m, a);
+        get8<kWide>(u + i, m, b);
+        to8(a, v);
+        to8(b, up);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) low = fminf(low, v[j]);
+        if (low < -80.0f) { /* there 1 + exp(-gate) leaves the reciprocal's range */
+#pragma unroll 1
+            for (int j = 0; j < m; ++j) {
+                const float w = (float)v64(i + j);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k == j) v[k] = w;
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float gate = v[j];
-            v[j] = __fmul_rn(__fdividef(gate, 1.0f + expf(-gate)), up[j]);
-            /* there 1 + exp(-gate) leaves what __fdividef takes */
-            if (gate < -80.0f) v[j] = (float)silu64((double)gate, (double)up[j]);
+            /* exp(-g) = 2^hi (1 + lo ln 2), hi + lo = -g log2 e */
+            constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147182f;
+            const float hi = __fmul_rn(v[j], -kLog2e);
+            const float lo = fmaf(v[j], -kLog2eLow, fmaf(v[j], -kLog2e, -hi));
+            float e, r;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
+            e = fmaf(__fmul_rn(e, lo), kLn2, e);
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, e)));
+            v[j] = __fmul_rn(__fmul_rn(v[j], r), up[j]);
         }
     }
     __device__ void again(int i, float (&v)[8]) const {
@@ -288,13 +326,14 @@ __device__ __forceinline__ double row_stat(RowShared &sh, int parts, int part, f
     }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    unsigned long long top = 0;
-    if (kNorm) sum = 0.0;
-    for (int i = 0; i < parts; ++i) {
-        top = max(top, sh.part_top[i]);
-        if (kNorm) sum += sh.part_sum[i];
+    const unsigned long long top = lane < parts ? sh.part_top[lane] : 0;
+    const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(top >> 32));
+    const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(top >> 32) == high ? (unsigned)top : 0u);
+    if (kNorm) {
+        sum = 0.0;
+        for (int i = 0; i < parts; ++i) sum += sh.part_sum[i];
     }
-    return of_bits(top);
+    return of_bits((unsigned long long)high << 32 | low);
 }
 
 /* A row's quantizer, once max|v| and the sum of squares are known. */
@@ -313,15 +352,21 @@ template <typename Row> struct RowQuant {
         if (Row::kNorm) about *= rsqrtf((float)sum * p.inv_n + p.eps);
         fits = about < 1e38f || top == 0.0 || top * factor(p) <= (double)kFltMax;
     }
+    /* 1.5 * 2^23: added, it leaves the nearest integer in the low bits */
+    static constexpr float kRound = 12582912.0f;
+    /* how far t may be from the nearest integer, u - kRound */
+    static __device__ __forceinline__ float off_centre(float t, float u) {
+        const float d = __fsub_rn(t, __fsub_rn(u, kRound));
+        return Row::kRelative > 0.0f ? fabsf(d) + fabsf(__fmul_rn(t, Row::kRelative)) : fabsf(d);
+    }
     /* q of the eight elements from i on */
     __device__ void store(const RowParams &p, const Row &row, int8_t *q, int i, const float (&v)[8]) const {
-        constexpr float kRound = 12582912.0f; /* 1.5 * 2^23: added, it leaves the nearest integer in the low bits */
         float u[8], far = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float t = __fmul_rn(v[j], r32);
             u[j] = __fadd_rn(t, kRound);
-            far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(u[j], kRound))));
+            far = fmaxf(far, off_centre(t, u[j]));
         }
         uint32_t w[2];
 #pragma unroll
@@ -330,16 +375,19 @@ template <typename Row> struct RowQuant {
                                __byte_perm(__float_as_uint(u[4 * h + 2]), __float_as_uint(u[4 * h + 3]), 0x0040), 0x5410);
         const bool none = !fits || top == 0.0;
         if (none) w[0] = w[1] = 0;
-        const int n = min(8, p.n - i);
-        put_q8(q + i, n, w);
+        const int n = Row::kWide ? 8 : min(8, p.n - i);
+        put_q8<Row::kWide>(q + i, n, w);
         if ((wide || !(far < 0.5f - Row::kBorder)) && !none) { /* next to a border: 64 bits decide */
-#pragma unroll 1
-            for (int j = 0; j < n; ++j) {
-                float t = 0.5f;
+            unsigned near = 0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (k == j) t = __fmul_rn(v[k], r32);
-                if (wide || !(fabsf(t - rintf(t)) < 0.5f - Row::kBorder)) q[i + j] = (int8_t)round64(row.v64(i + j), top);
+            for (int j = 0; j < 8; ++j) {
+                const float t = __fmul_rn(v[j], r32);
+                near |= (wide || !(off_centre(t, __fadd_rn(t, kRound)) < 0.5f - Row::kBorder) ? 1u : 0u) << j;
+            }
+            near &= (1u << n) - 1u;
+            for (; near != 0; near &= near - 1) {
+                const int j = i + __ffs(near) - 1;
+                q[j] = (int8_t)round64(row.v64(j), top);
             }
         }
     }
@@ -445,7 +493,7 @@ cudaError_t launch_parts(RowParams p, int rows, int parts, cudaStream_t st) {
 }
 
 constexpr int kFewN = 8192, kFewPart = 2048;
-template <typename Row> cudaError_t launch_rows(RowParams p, int rows, int num_sms, cudaStream_t st) {
+template <typename Row> cudaError_t launch_row(RowParams p, int rows, int num_sms, cudaStream_t st) {
     p.inv_n = 1.0f / (float)p.n;
     /* Few rows: a thread takes 8 elements, and a long row is spread over as
      * many SMs as a cluster has.  Many: 16 elements, and no more CTAs a row
@@ -454,10 +502,21 @@ template <typename Row> cudaError_t launch_rows(RowParams p, int rows, int num_s
         if (p.n <= kFewN) return launch_parts<Row, 1, 1024, 1>(p, rows, 1, st);
         if (p.n <= kMaxParts * 8192) return launch_parts<Row, 1, 1024, 1>(p, rows, std::min(kMaxParts, (p.n + kFewPart - 1) / kFewPart), st);
     } else if (p.n <= kMaxParts * 8192 && rows <= 0x7fffffff / kMaxParts) {
-        return launch_parts<Row, 2, 512, 2>(p, rows, (p.n + 8191) / 8192, st);
+        if (Row::kNorm) return launch_parts<Row, 2, 512, 2>(p, rows, (p.n + 8191) / 8192, st);
+        if (p.n <= kMaxParts * 4096) return launch_parts<Row, 2, 256, 5>(p, rows, (p.n + 4095) / 4096, st);
     }
     row_q8_long_kernel<Row><<<rows, kLongThreads, 0, st>>>(p);
     return cudaGetLastError();
+}
+
+/* kWide where every row of every buffer begins at a 16-byte boundary (q: 8)
+ * and ends at a whole eight: no test of alignment or of the end an element. */
+template <template <typename, bool> class Row, typename T>
+cudaError_t launch_rows(const RowParams &p, int rows, int num_sms, cudaStream_t st) {
+    const long long strides = p.a_stride | p.b_stride | (p.h != nullptr ? p.h_stride : 0);
+    const bool wide = p.n % 8 == 0 && (((uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.h | (uintptr_t)p.w) & 15) == 0 &&
+                      strides * (long long)sizeof(T) % 16 == 0 && ((uintptr_t)p.q | (uintptr_t)p.q_stride) % 8 == 0;
+    return wide ? launch_row<Row<T, true>>(p, rows, num_sms, st) : launch_row<Row<T, false>>(p, rows, num_sms, st);
 }
 
 }  // namespace
@@ -502,9 +561,9 @@ int lal_tail_add_rms_norm_q8(const void *d_x, int64_t x_stride, const void *d_re
     const RowParams p = {d_x, d_residual, d_h, d_norm_w, x_stride, residual_stride, h_stride, q_stride,
                          n_embd, eps, d_q, d_scale, 1, 0.0f};
     cudaStream_t st = (cudaStream_t)stream;
-    return launched(op, dtype == LAL_TAIL_F32    ? launch_rows<NormRow<float>>(p, rows, dev.num_sms(), st)
-                        : dtype == LAL_TAIL_BF16 ? launch_rows<NormRow<__nv_bfloat16>>(p, rows, dev.num_sms(), st)
-                                                 : launch_rows<NormRow<__half>>(p, rows, dev.num_sms(), st));
+    return launched(op, dtype == LAL_TAIL_F32    ? launch_rows<NormRow, float>(p, rows, dev.num_sms(), st)
+                        : dtype == LAL_TAIL_BF16 ? launch_rows<NormRow, __nv_bfloat16>(p, rows, dev.num_sms(), st)
+                                                 : launch_rows<NormRow, __half>(p, rows, dev.num_sms(), st));
 }
 
 int lal_tail_swiglu_q8(const void *d_gate, int64_t gate_stride, const void *d_up, int64_t up_stride,
@@ -532,9 +591,9 @@ int lal_tail_swiglu_q8(const void *d_gate, int64_t gate_stride, const void *d_up
     const RowParams p = {d_gate, d_up, nullptr, nullptr, gate_stride, up_stride, 0, q_stride,
                          n, 0.0f, d_q, d_scale, 1, 0.0f};
     cudaStream_t st = (cudaStream_t)stream;
-    return launched(op, dtype == LAL_TAIL_F32    ? launch_rows<SwigluRow<float>>(p, rows, dev.num_sms(), st)
-                        : dtype == LAL_TAIL_BF16 ? launch_rows<SwigluRow<__nv_bfloat16>>(p, rows, dev.num_sms(), st)
-                                                 : launch_rows<SwigluRow<__half>>(p, rows, dev.num_sms(), st));
+    return launched(op, dtype == LAL_TAIL_F32    ? launch_rows<SwigluRow, float>(p, rows, dev.num_sms(), st)
+                        : dtype == LAL_TAIL_BF16 ? launch_rows<SwigluRow, __nv_bfloat16>(p, rows, dev.num_sms(), st)
+                                                 : launch_rows<SwigluRow, __half>(p, rows, dev.num_sms(), st));
 }
 
 }  // extern "C"
