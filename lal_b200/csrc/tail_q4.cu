@@ -249,18 +249,8 @@ struct MatvecParams {
  * carry 1/16.  The dots of a group are exact int32 (below 2^24), and are
  * scaled and added in fp32.  With a minimum, w = s (q - 8) + (8 s + m): a
  * second product with rows of 16 gives 16 times the sums of the vectors. */
-constexpr int kMmaWarps = 8;
-constexpr int kMmaStreams = 8;
 constexpr int kStageBlocks = 8;               /* 256 columns */
-constexpr int kStageARow = kStageBlocks * 16; /* block k of row r in place k ^ (r mod 8): no bank conflicts */
-constexpr int kStageA = 16 * kStageARow;
-constexpr int kStageS = 2 * 16 * 2 * kStageBlocks; /* scales and minima, groups of 32 */
-constexpr int kStageXRow = kStageBlocks * 32 + 16; /* rows 16 bytes apart mod 128 */
-constexpr int kMmaSmem = 113 * 1024 - 1024; /* two CTAs an SM */
-static_assert(kMmaWarps * 3 * (kStageA + kStageS + 8 * kStageXRow) <= kMmaSmem, "up to eight streams, three stages");
-static_assert(kMmaWarps * 4 * (kStageA + kStageS + 3 * kStageXRow) <= kMmaSmem, "up to three streams, four stages");
-
-/* 16 (or 4) bytes to shared memory, the last 16 - n of them zeros */
+/* 16 bytes to shared memory, the last 16 - n of them zeros */
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int n) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
@@ -275,6 +265,13 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+/* the same from zero */
+__device__ __forceinline__ void mma_s8_zero(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
 }
 
 /* n (0 to 16) columns c0 .. of a vector's row to 16 bytes of shared memory,
@@ -318,321 +315,260 @@ __device__ __forceinline__ void store_y(const MatvecParams &p, int b, int row, f
         ((__half *)p.y)[at] = __float2half_rn(v);
 }
 
-/* ---- one or two streams: 4-way int8 dot products ----
- *
- * A warp takes kR rows; a lane takes every 32nd block of each (16 bytes, all
- * kR loads at once), eight dp4a a block and stream, and one scaled addition
- * in fp32.  The vectors lie in shared memory as two planes, columns 0-15 and
- * 16-31 of the blocks, so that a warp's 16-byte reads have no bank conflicts.
- * With few rows the K range of a row is split over warps of the CTA. */
-constexpr int kDotWarps = 8;
-
-template <int kB, int kR, bool kMin>
-__global__ void __launch_bounds__(32 * kDotWarps) q4_dot_kernel(const MatvecParams p, int warps_k, int group_shift) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nb = q4_blocks(p.cols), groups = ((nb - 1) >> group_shift) + 1;
-    uint4 *xs = (uint4 *)smem; /* [kB][2][nb] */
-    int *sums = (int *)(smem + (size_t)kB * nb * 32); /* [kB][nb] */
-    const bool x_aligned = (((uintptr_t)p.x | (uintptr_t)p.x_stride) & 15) == 0;
-    for (int c = threadIdx.x; c < kB * nb * 2; c += 32 * kDotWarps) {
-        const int b = kB == 1 ? 0 : c / (nb * 2), i = c - b * nb * 2;
-        stage_x16((uint8_t *)(xs + (size_t)(b * 2 + (i & 1)) * nb + (i >> 1)), p.x + b * p.x_stride, i * 16, p.cols,
-                  x_aligned);
-    }
-    const int wk = warp % warps_k;
-    const int row0 = (blockIdx.x * (kDotWarps / warps_k) + warp / warps_k) * kR;
-    const uint4 *q[kR];
-    const __half *s[kR], *m[kR];
+/* A warp's results from mma accumulators: 16 kMT rows from row0 (`rows` of them
+ * exist) by 8 kNT streams from b0 (nx exist).  Written out once for each type,
+ * with addresses moved on: code that runs once a tile is fetched for it alone. */
+template <typename T, int kMT, int kNT>
+__device__ __forceinline__ void store_tile_as(const MatvecParams &p, int b0, int nx, int row0, int rows,
+                                              const float (&acc)[kMT][kNT][4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    T *y = (T *)p.y + (size_t)(b0 + 2 * t) * p.y_stride + row0 + g;
+    const float *sx = p.sx + b0 + 2 * t;
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-        const int row = min(row0 + r, p.rows - 1);
-        q[r] = (const uint4 *)p.q + (size_t)row * nb;
-        s[r] = p.scale + (size_t)row * groups;
-        m[r] = p.min + (size_t)row * groups;
-    }
-    cp_async_commit();
-    cp_async_wait<0>();
-    __syncthreads();
-    if (kMin) {
-        for (int c = threadIdx.x; c < kB * nb; c += 32 * kDotWarps) {
-            const int b = kB == 1 ? 0 : c / nb, i = c - b * nb;
-            const uint4 lo = xs[(size_t)(b * 2) * nb + i], hi = xs[(size_t)(b * 2 + 1) * nb + i];
-            int sum = 0;
-            for (uint32_t v : {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}) sum = __dp4a((int)v, 0x10101010, sum);
-            sums[c] = sum; /* 16 times the sum, as the dots */
-        }
-        __syncthreads();
-    }
-    float acc[kR][kB] = {};
-    constexpr int kU = kR >= 4 ? 1 : 4 / kR; /* blocks of a row in flight */
-    if (row0 < p.rows) {
-        for (int k0 = wk * 32 + lane; k0 < nb; k0 += 32 * kU * warps_k) {
-            uint4 v[kU][kR];
-            float sc[kU][kR], lo[kU][kR];
+    for (int n = 0; n < kNT; ++n, y += 8 * p.y_stride) {
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int k = k0 + 32 * u * warps_k;
+        for (int c = 0; c < 2; ++c) {
+            if (8 * n + 2 * t + c >= nx) break;
+            const float s = __ldg(sx + 8 * n + c);
 #pragma unroll
-                for (int r = 0; r < kR; ++r) {
-                    if (k >= nb) break;
-                    v[u][r] = __ldg(q[r] + k);
-                    sc[u][r] = __half2float(__ldg(s[r] + (k >> group_shift)));
-                    if (kMin) lo[u][r] = __half2float(__ldg(m[r] + (k >> group_shift)));
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int k = k0 + 32 * u * warps_k;
-                if (k >= nb) break;
-#pragma unroll
-                for (int b = 0; b < kB; ++b) {
-                    const uint4 xl = xs[(size_t)(b * 2) * nb + k], xh = xs[(size_t)(b * 2 + 1) * nb + k];
-                    const uint32_t x0[4] = {xl.x, xl.y, xl.z, xl.w}, x1[4] = {xh.x, xh.y, xh.z, xh.w};
-                    const float sum = kMin ? (float)sums[b * nb + k] : 0.0f;
-#pragma unroll
-                    for (int r = 0; r < kR; ++r) {
-                        const uint32_t w[4] = {v[u][r].x, v[u][r].y, v[u][r].z, v[u][r].w};
-                        int dot = 0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            dot = __dp4a((int)(((w[i] << 4) & 0xf0f0f0f0u) ^ 0x80808080u), (int)x0[i], dot);
-                            dot = __dp4a((int)((w[i] & 0xf0f0f0f0u) ^ 0x80808080u), (int)x1[i], dot);
-                        }
-                        acc[r][b] = fmaf(sc[u][r], (float)dot, acc[r][b]);
-                        if (kMin) acc[r][b] = fmaf(fmaf(8.0f, sc[u][r], lo[u][r]), sum, acc[r][b]);
-                    }
-                }
-            }
+            for (int r = 0; r < 2 * kMT; ++r)
+                if (g + 8 * r < rows)
+                    y[c * p.y_stride + 8 * r] = from_f32<T>(__fmul_rn(s, __fmul_rn(0.0625f, acc[r >> 1][n][2 * (r & 1) + c])));
         }
     }
-#pragma unroll
-    for (int r = 0; r < kR; ++r)
-#pragma unroll
-        for (int b = 0; b < kB; ++b) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) acc[r][b] += __shfl_xor_sync(0xffffffffu, acc[r][b], o);
-            acc[r][b] *= 0.0625f;
-        }
-    if (warps_k == 1) {
-        if (lane == 0)
-#pragma unroll
-            for (int r = 0; r < kR; ++r)
-#pragma unroll
-                for (int b = 0; b < kB; ++b)
-                    if (row0 + r < p.rows) store_y(p, b, row0 + r, acc[r][b]);
-        return;
-    }
-    /* the warps of a row, in order */
-    __shared__ float part[kDotWarps][kR * kB];
-    if (lane == 0)
-#pragma unroll
-        for (int i = 0; i < kR * kB; ++i) part[warp][i] = acc[i / kB][i % kB];
-    __syncthreads();
-    const int tiles = kDotWarps / warps_k;
-    for (int i = threadIdx.x; i < tiles * kR * kB; i += 32 * kDotWarps) {
-        const int tile = i / (kR * kB), j = i % (kR * kB);
-        const int row = (blockIdx.x * tiles + tile) * kR + j / kB;
-        float sum = 0.0f;
-        for (int w = 0; w < warps_k; ++w) sum += part[tile * warps_k + w][j];
-        if (row < p.rows) store_y(p, j % kB, row, sum);
-    }
+}
+template <int kMT, int kNT>
+__device__ __forceinline__ void store_tile(const MatvecParams &p, int b0, int nx, int row0, int rows,
+                                           const float (&acc)[kMT][kNT][4]) {
+    if (p.dtype == LAL_TAIL_F32) store_tile_as<float>(p, b0, nx, row0, rows, acc);
+    else if (p.dtype == LAL_TAIL_BF16) store_tile_as<__nv_bfloat16>(p, b0, nx, row0, rows, acc);
+    else store_tile_as<__half>(p, b0, nx, row0, rows, acc);
 }
 
-constexpr int kDotSmem = 96 * 1024;
-
-inline int dot_smem(const MatvecParams &p, int streams) {
-    const long long n = (long long)streams * q4_blocks(p.cols) * (32 + (p.min ? 4 : 0));
-    return n > kDotSmem ? -1 : (int)n;
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
 }
 
-template <int kB, int kR, bool kMin> cudaError_t launch_dot(const MatvecParams &p, int num_sms, cudaStream_t st) {
-    const int nb = q4_blocks(p.cols), tiles = (p.rows + kR - 1) / kR;
-    int wk = 1;
-    while (wk < kDotWarps && 32 * wk < nb && (long long)tiles * wk < 16LL * num_sms) wk *= 2;
-    const void *fn = (const void *)q4_dot_kernel<kB, kR, kMin>;
-    cudaError_t e = raise_smem(fn, kDotSmem);
-    if (e != cudaSuccess) return e;
-    const int per = kDotWarps / wk, shift = p.group == 32 ? 0 : p.group == 64 ? 1 : 2;
-    q4_dot_kernel<kB, kR, kMin><<<(tiles + per - 1) / per, 32 * kDotWarps, dot_smem(p, kB), st>>>(p, wk, shift);
-    return cudaGetLastError();
-}
+/* Stages of a warp's ring, warps of a CTA, CTAs of an SM.  kMany (32 rows by 16
+ * streams, tiles for several waves): more warps with shorter rings; 62 us
+ * against 74 for 152064x3584 and sixteen streams, but 30 against 17 for
+ * 37888x3584, one wave. */
+constexpr int mma_depth(bool many) { return many ? 2 : 3; }
+constexpr int mma_warps(bool many) { return many ? 12 : 8; }
+constexpr int mma_ctas(int mt, int nt) { return mt * nt == 1 ? 2 : 1; }
 
-template <int kB> cudaError_t launch_dot(const MatvecParams &p, int num_sms, cudaStream_t st) {
-    /* rows a warp: four once that leaves 24 warps an SM */
-    const int per_warp = p.rows / (24 * num_sms);
-    if (p.min)
-        return per_warp >= 4   ? launch_dot<kB, 4, true>(p, num_sms, st)
-               : per_warp >= 2 ? launch_dot<kB, 2, true>(p, num_sms, st)
-                               : launch_dot<kB, 1, true>(p, num_sms, st);
-    return per_warp >= 4   ? launch_dot<kB, 4, false>(p, num_sms, st)
-           : per_warp >= 2 ? launch_dot<kB, 2, false>(p, num_sms, st)
-                           : launch_dot<kB, 1, false>(p, num_sms, st);
-}
+/* What a warp's ring holds a stage: weights of 16 kMT rows, their scales (and
+ * minima), the part of 8 kNT vectors. */
+template <int kMT, int kNT, int kGroup, bool kMin, bool kMany> struct MmaStage {
+    static constexpr int kGroups = kStageBlocks * kQ4Block / kGroup;
+    static constexpr int kScale = 16 * kMT * kGroups * 2;
+    static constexpr int kS = 16 * kMT * 128, kX = (kS + (kMin ? 2 : 1) * kScale + 127) / 128 * 128;
+    static constexpr int kBytes = (kX + 8 * kNT * kStageBlocks * 32 + 127) / 128 * 128;
+    static constexpr int kDepth = mma_depth(kMany), kWarps = mma_warps(kMany), kCtas = mma_ctas(kMT, kNT);
+    static constexpr int kSmem = kWarps * kDepth * kBytes;
+    static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "CTAs of an SM");
+};
 
-template <int kGroup, bool kMin, int kDepth>
-__global__ void __launch_bounds__(32 * kMmaWarps, 2) q4_mma_kernel(const MatvecParams p, int warps_k) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    constexpr int kPer = kGroup / kQ4Block;             /* blocks of a group */
-    constexpr int kGroups = kStageBlocks / kPer;        /* groups of a stage */
+template <int kMT, int kNT, int kGroup, bool kMin, bool kMany>
+__global__ void __launch_bounds__(32 * mma_warps(kMany), mma_ctas(kMT, kNT)) q4_mma_kernel(const MatvecParams p, int x_base, int warps_k, int height) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    using Stage = MmaStage<kMT, kNT, kGroup, kMin, kMany>;
+    constexpr int kDepth = Stage::kDepth, kWarps = Stage::kWarps;
+    constexpr int kPer = kGroup / kQ4Block, kGroups = Stage::kGroups; /* blocks of a group, groups of a stage */
+    constexpr int kRows = 16 * kMT, kStreams = 8 * kNT;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int wk = warp % warps_k;
-    const int row0 = (blockIdx.x * (kMmaWarps / warps_k) + warp / warps_k) * 16;
-    const int b0 = blockIdx.y * kMmaStreams, nx = min(kMmaStreams, p.streams - b0);
+    const int row0 = (blockIdx.x * (kWarps / warps_k) + warp / warps_k) * height;
+    const int b0 = x_base + blockIdx.y * kStreams, nx = min(kStreams, p.streams - b0);
     const int nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
     const int stages = (nb + kStageBlocks - 1) / kStageBlocks;
-    const int stage_bytes = kStageA + kStageS + min(kMmaStreams, p.streams) * kStageXRow;
-    uint8_t *ring = smem + warp * kDepth * stage_bytes;
+    uint8_t *const ring = smem + warp * kDepth * Stage::kBytes;
+    const uint32_t ring32 = smem_u32(ring);
 
-    float acc[4] = {};
+    float acc[kMT][kNT][4] = {};
     const bool live = row0 < p.rows;
     if (live) {
-        /* this lane's share of a stage: four 16-byte blocks of weights, up to four of the vectors */
-        const uint8_t *qsrc[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            qsrc[j] = p.q + ((size_t)min(row0 + (lane >> 3) + 4 * j, p.rows - 1) * nb + (lane & 7)) * 16;
-        const uint32_t qdst = (lane >> 3) * kStageARow + ((lane & 7) ^ (lane >> 3)) * 16;
-        const int8_t *xrow = p.x + (size_t)(b0 + min(lane >> 4, nx - 1)) * p.x_stride;
+        const int rows = min(height, p.rows - row0);
+        /* ---- loads: this lane's share of a stage, its sources moved on by warps_k stages ---- */
+        /* block lane & 7 of rows lane / 8, + 4, ...; in place block ^ (row mod 8) */
+        const int w_r = lane >> 3, w_k = lane & 7;
+        const uint32_t w_to = ring32 + w_r * 128 + ((w_k ^ w_r) << 4);
+        const uint8_t *w_src = p.q + ((size_t)(row0 + w_r) * nb + wk * kStageBlocks + w_k) * 16;
+        const size_t w_step = (size_t)nb * 64;
+        /* 16 bytes lane & 15 of vectors lane / 16, + 2, ...; in place piece ^ (vector mod 8) */
+        const int x_n = lane >> 4, x_c = lane & 15;
+        const int8_t *x_src = p.x + (size_t)(b0 + x_n) * p.x_stride;
+        const size_t x_step = (size_t)2 * p.x_stride;
         const bool x_aligned = (((uintptr_t)p.x | (uintptr_t)p.x_stride) & 15) == 0;
-        /* scales of lane's row, kGroups a stage: one copy where every row's are aligned to it */
-        const unsigned short *ssrc = (const unsigned short *)(lane < 16 ? p.scale : p.min) +
-                                     (size_t)min(row0 + (lane & 15), p.rows - 1) * groups;
-        const bool s_aligned = ((((uintptr_t)p.scale | (kMin ? (uintptr_t)p.min : 0) | (uintptr_t)(groups * 2)) & (2 * kGroups - 1)) == 0);
+        /* a row's scales of a stage, one copy where all rows' are aligned to it: lane has row lane (+ 16: a minimum's) */
+        constexpr int kCopies = kRows * (kMin ? 2 : 1);
+        const bool s_aligned =
+            (((uintptr_t)p.scale | (kMin ? (uintptr_t)p.min : 0) | (uintptr_t)(groups * 2)) & (2 * kGroups - 1)) == 0;
         auto load = [&](int st, int slot) {
-            uint8_t *a = ring + slot * stage_bytes;
+            const uint32_t base = slot * Stage::kBytes;
             const int k0 = st * kStageBlocks;
-            const bool in = k0 + (lane & 7) < nb;
+            if (k0 + w_k < nb) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                cp_async16(smem_u32(a + ((qdst + 4 * j * kStageARow) ^ (j & 1 ? 64 : 0))), in ? qsrc[j] + (size_t)k0 * 16 : p.q, in ? 16 : 0);
-            if (kMin || lane < 16) {
-                /* [16 rows][kGroups] scales, then minima */
-                unsigned short *d = (unsigned short *)(a + kStageA) + lane * kGroups;
-                const int g0 = st * kGroups;
+                for (int j = 0; j < 4 * kMT; ++j)
+                    if (w_r + 4 * j < rows) cp_async16((w_to + base + j * 512) ^ (j & 1 ? 64 : 0), w_src + j * w_step, 16);
+            }
+            w_src += (size_t)warps_k * (kStageBlocks * 16);
+            const int c0 = k0 * kQ4Block + x_c * 16;
+            uint8_t *const x_to = ring + base + Stage::kX + x_n * 256;
+            const int8_t *x = x_src;
+            if (x_aligned && c0 + 16 <= p.cols) {
+#pragma unroll
+                for (int j = 0; j < 4 * kNT; ++j, x += x_step)
+                    if (x_n + 2 * j < nx)
+                        cp_async16_l1(smem_u32(x_to + j * 512 + ((x_c ^ ((x_n + 2 * j) & 7)) << 4)), x + c0, 16);
+            } else {
+#pragma unroll 1
+                for (int j = 0; x_n + 2 * j < nx; ++j, x += x_step)
+                    stage_x16(x_to + j * 512 + ((x_c ^ ((x_n + 2 * j) & 7)) << 4), x, c0, p.cols, x_aligned);
+            }
+            const int g0 = st * kGroups;
+#pragma unroll
+            for (int i = lane; i < kCopies; i += 32) {
+                const int r = i % kRows;
+                const unsigned short *src =
+                    (const unsigned short *)(i < kRows ? p.scale : p.min) + (size_t)(row0 + min(r, rows - 1)) * groups + g0;
+                unsigned short *to = (unsigned short *)(ring + base + Stage::kS) + i * kGroups;
                 if (s_aligned && g0 + kGroups <= groups) {
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(d)), "l"(ssrc + g0),
-                                 "n"(2 * kGroups)
-                                 : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(src), "n"(2 * kGroups) : "memory");
                 } else {
 #pragma unroll
-                    for (int i = 0; i < kGroups; ++i)
-                        if (g0 + i < groups) d[i] = __ldg(ssrc + g0 + i);
+                    for (int k = 0; k < kGroups; ++k) to[k] = g0 + k < groups ? __ldg(src + k) : 0;
                 }
             }
-            const int8_t *xr = xrow;
-            for (int c = lane; c < nx * 16; c += 32, xr += 2 * p.x_stride)
-                stage_x16(a + kStageA + kStageS + (c >> 4) * kStageXRow + (c & 15) * 16, xr,
-                          k0 * kQ4Block + (c & 15) * 16, p.cols, x_aligned);
         };
+        int ahead = wk;
 #pragma unroll
-        for (int i = 0; i < kDepth - 1; ++i) {
-            if (wk + i * warps_k < stages) load(wk + i * warps_k, i);
+        for (int i = 0; i < kDepth - 1; ++i, ahead += warps_k) {
+            if (ahead < stages) load(ahead, i);
             cp_async_commit();
         }
+        /* ldmatrix addresses: rows lane mod 16, block lane / 16 of a pair; vectors lane mod 8, piece lane / 8 of a pair's four */
+        const uint32_t a_at = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+        const uint32_t x_at = Stage::kX + (lane & 7) * 256 + (((lane >> 3) ^ (lane & 7)) << 4);
         int slot = 0;
-        const int xg = min(g, nx - 1); /* vectors that are not there: any, their sums are dropped */
-        for (int st = wk; st < stages; st += warps_k) {
+        for (int st = wk; st < stages; st += warps_k, ahead += warps_k) {
             cp_async_wait<kDepth - 2>();
             __syncwarp();
-            {
-                const int next = st + (kDepth - 1) * warps_k;
-                if (next < stages) load(next, slot == 0 ? kDepth - 1 : slot - 1);
-                cp_async_commit();
-            }
-            const uint8_t *a = ring + slot * stage_bytes + g * kStageARow + 4 * t;
-            const uint32_t turn = g * 16;
-            const uint8_t *x = ring + slot * stage_bytes + kStageA + kStageS + xg * kStageXRow + 4 * t;
-            /* the scales (and minima) of rows g and g + 8 */
+            if (ahead < stages) load(ahead, slot == 0 ? kDepth - 1 : slot - 1);
+            cp_async_commit();
+            const uint32_t at = ring32 + slot * Stage::kBytes;
             using Pack = std::conditional_t<kGroups == 8, uint4, std::conditional_t<kGroups == 4, uint2, uint32_t>>;
-            const Pack *sc = (const Pack *)(ring + slot * stage_bytes + kStageA) + g;
             union Row {
                 Pack all;
                 __half one[kGroups];
                 __device__ Row() {}
-            } scale[2], low[2];
+            } scale[kMT][2], low[kMT][2]; /* of rows g and g + 8 */
+            const Pack *sc = (const Pack *)(ring + slot * Stage::kBytes + Stage::kS) + g;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                scale[h].all = sc[8 * h];
-                if (kMin) low[h].all = sc[16 + 8 * h];
-            }
-            const int left = nb - st * kStageBlocks; /* blocks from this stage on */
-#pragma unroll
-            for (int gr = 0; gr < kGroups; ++gr) {
-                if (gr * kPer >= left) break;
-                int c[4] = {}, cx[4] = {};
-#pragma unroll
-                for (int k = gr * kPer; k < (gr + 1) * kPer; ++k) {
-                    /* blocks behind the row's end hold zeros in the vectors */
-                    const uint32_t w0 = *(const uint32_t *)(a + (k * 16 ^ turn)),
-                                   w1 = *(const uint32_t *)(a + 8 * kStageARow + (k * 16 ^ turn));
-                    const uint32_t x0 = *(const uint32_t *)(x + k * 32), x1 = *(const uint32_t *)(x + k * 32 + 16);
-                    const uint32_t av[4] = {((w0 << 4) & 0xf0f0f0f0u) ^ 0x80808080u, ((w1 << 4) & 0xf0f0f0f0u) ^ 0x80808080u,
-                                            (w0 & 0xf0f0f0f0u) ^ 0x80808080u, (w1 & 0xf0f0f0f0u) ^ 0x80808080u};
-                    mma_s8(c, av, x0, x1);
-                    if (kMin) {
-                        const uint32_t ones[4] = {0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u};
-                        mma_s8(cx, ones, x0, x1);
-                    }
-                }
+            for (int m = 0; m < kMT; ++m)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float s = __half2float(scale[h].one[gr]);
+                    scale[m][h].all = sc[16 * m + 8 * h];
+                    if (kMin) low[m][h].all = sc[kRows + 16 * m + 8 * h];
+                }
+            int c[kMT][kNT][4], cx[kNT][4];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) acc[2 * h + i] = fmaf(s, (float)c[2 * h + i], acc[2 * h + i]);
+            for (int pair = 0; pair < kStageBlocks / 2; ++pair) {
+                /* blocks behind the row's end hold zeros in the vectors, and their groups scales of zero */
+                uint32_t w[kMT][4], x[kNT][4];
+#pragma unroll
+                for (int m = 0; m < kMT; ++m) ldmatrix4(w[m], (at + a_at + m * 2048) ^ (pair << 5));
+#pragma unroll
+                for (int n = 0; n < kNT; ++n) ldmatrix4(x[n], ((at + x_at + n * 2048) ^ ((pair & 1) << 6)) + (pair >> 1) * 128);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int block = 2 * pair + k;
+                    const bool begin = block % kPer == 0;
                     if (kMin) {
-                        const float m = fmaf(8.0f, s, __half2float(low[h].one[gr]));
+                        const uint32_t ones[4] = {0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u};
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) acc[2 * h + i] = fmaf(m, (float)cx[i], acc[2 * h + i]);
+                        for (int n = 0; n < kNT; ++n) {
+                            if (begin) mma_s8_zero(cx[n], ones, x[n][2 * k], x[n][2 * k + 1]);
+                            else mma_s8(cx[n], ones, x[n][2 * k], x[n][2 * k + 1]);
+                        }
+                    }
+#pragma unroll
+                    for (int m = 0; m < kMT; ++m) {
+                        const uint32_t w0 = w[m][2 * k], w1 = w[m][2 * k + 1];
+                        const uint32_t a[4] = {((w0 << 4) & 0xf0f0f0f0u) ^ 0x80808080u, ((w1 << 4) & 0xf0f0f0f0u) ^ 0x80808080u,
+                                               (w0 & 0xf0f0f0f0u) ^ 0x80808080u, (w1 & 0xf0f0f0f0u) ^ 0x80808080u};
+#pragma unroll
+                        for (int n = 0; n < kNT; ++n) {
+                            if (begin) mma_s8_zero(c[m][n], a, x[n][2 * k], x[n][2 * k + 1]);
+                            else mma_s8(c[m][n], a, x[n][2 * k], x[n][2 * k + 1]);
+                        }
+                        if (block % kPer != kPer - 1) continue;
+                        const int gr = block / kPer;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float s = __half2float(scale[m][h].one[gr]);
+                            const float l = kMin ? fmaf(8.0f, s, __half2float(low[m][h].one[gr])) : 0.0f;
+#pragma unroll
+                            for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    acc[m][n][2 * h + i] = fmaf(s, (float)c[m][n][2 * h + i], acc[m][n][2 * h + i]);
+                                    if (kMin) acc[m][n][2 * h + i] = fmaf(l, (float)cx[n][i], acc[m][n][2 * h + i]);
+                                }
+                        }
                     }
                 }
             }
             slot = slot + 1 == kDepth ? 0 : slot + 1;
         }
         cp_async_wait<0>();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] *= 0.0625f;
     }
     if (warps_k == 1) {
-        if (live)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = row0 + g + (i >> 1) * 8, b = 2 * t + (i & 1);
-                if (row < p.rows && b < nx) store_y(p, b0 + b, row, acc[i]);
-            }
+        if (live) store_tile(p, b0, nx, row0, min(height, p.rows - row0), acc);
         return;
     }
     /* the warps of a row tile, in order; their sums take the rings' place */
     __syncthreads();
-    float(*part)[16 * kMmaStreams] = (float(*)[16 * kMmaStreams])smem;
+    float(*part)[kRows * kStreams] = (float(*)[kRows * kStreams])smem;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[warp][(2 * t + (i & 1)) * 16 + g + (i >> 1) * 8] = acc[i];
+    for (int m = 0; m < kMT; ++m)
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                part[warp][(8 * n + 2 * t + (i & 1)) * kRows + 16 * m + g + (i >> 1) * 8] = acc[m][n][i];
     __syncthreads();
-    const int tiles = kMmaWarps / warps_k;
-    for (int i = threadIdx.x; i < tiles * 16 * nx; i += 32 * kMmaWarps) {
-        const int r = i & 15, b = (i >> 4) % nx, tile = (i >> 4) / nx;
-        const int row = (blockIdx.x * tiles + tile) * 16 + r;
-        if (row >= p.rows) continue;
+    const int tiles = kWarps / warps_k;
+    for (int i = threadIdx.x; i < tiles * kRows * nx; i += 32 * kWarps) {
+        const int r = i % kRows, b = i / kRows % nx, tile = i / kRows / nx;
+        const int row = (blockIdx.x * tiles + tile) * height + r;
+        if (r >= height || row >= p.rows) continue;
         float sum = 0.0f;
-        for (int w = 0; w < warps_k; ++w) sum += part[tile * warps_k + w][b * 16 + r];
-        store_y(p, b0 + b, row, sum);
+        for (int w = 0; w < warps_k; ++w) sum += part[tile * warps_k + w][b * kRows + r];
+        store_y(p, b0 + b, row, 0.0625f * sum);
     }
 }
 
-template <int kGroup, bool kMin, int kDepth>
-cudaError_t launch_mma(const MatvecParams &p, int num_sms, cudaStream_t st) {
-    /* warps of a row tile: enough that the tiles' warps fill the SMs (16 a SM),
-     * no more than there are stages */
-    const int tiles = (p.rows + 15) / 16, stages = (q4_blocks(p.cols) + kStageBlocks - 1) / kStageBlocks;
+template <int kMT, int kNT, int kGroup, bool kMin, bool kMany>
+cudaError_t launch_mma(const MatvecParams &p, int x_base, int num_sms, cudaStream_t st) {
+    /* warps of a row tile: enough that the tiles' warps fill the SMs, no more than there are stages */
+    using Stage = MmaStage<kMT, kNT, kGroup, kMin, kMany>;
+    constexpr int kRows = 16 * kMT, kWarps = Stage::kWarps, kWarpsSm = Stage::kCtas * kWarps;
+    const int tiles = (p.rows + kRows - 1) / kRows, stages = (q4_blocks(p.cols) + kStageBlocks - 1) / kStageBlocks;
     int wk = 1;
-    while (wk < kMmaWarps && 2 * wk <= stages && (long long)tiles * wk < 16LL * num_sms) wk *= 2;
-    const int smem = kMmaWarps * kDepth * (kStageA + kStageS + std::min(kMmaStreams, p.streams) * kStageXRow);
-    const void *fn = (const void *)q4_mma_kernel<kGroup, kMin, kDepth>;
-    cudaError_t e = raise_smem(fn, kMmaSmem);
+    while (!kMany && wk < kWarps && 2 * wk <= stages && (long long)tiles * wk < (long long)kWarpsSm * num_sms) wk *= 2;
+    /* rows of a tile: fewer than it holds where that gives every SM some */
+    const int at_once = num_sms * (kWarpsSm / wk), waves = (tiles + at_once - 1) / at_once;
+    const int height = waves > 1 ? kRows : std::max((p.rows + at_once - 1) / at_once, std::min(p.rows, kRows / 2));
+    const int n = (p.rows + height - 1) / height, per = kWarps / wk;
+    constexpr int smem = Stage::kSmem;
+    const cudaError_t e = raise_smem((const void *)q4_mma_kernel<kMT, kNT, kGroup, kMin, kMany>, smem);
     if (e != cudaSuccess) return e;
-    const int per = kMmaWarps / wk;
-    q4_mma_kernel<kGroup, kMin, kDepth>
-        <<<dim3((tiles + per - 1) / per, (p.streams + kMmaStreams - 1) / kMmaStreams), 32 * kMmaWarps, smem, st>>>(p, wk);
+    q4_mma_kernel<kMT, kNT, kGroup, kMin, kMany>
+        <<<dim3((n + per - 1) / per, (p.streams - x_base + 8 * kNT - 1) / (8 * kNT)), 32 * kWarps, smem, st>>>(p, x_base, wk, height);
     return cudaGetLastError();
 }
 
@@ -656,15 +592,17 @@ cudaError_t launch_mma(const MatvecParams &p, int num_sms, cudaStream_t st) {
 constexpr int kTcUnpack = 8, kTcEpi = 16, kTcLoad = 4;
 constexpr int kTcIssue = kTcUnpack + kTcEpi; /* the warp that issues the products */
 constexpr int kTcWarps = kTcIssue + 1 + kTcLoad;
+constexpr int kTcA = 4;        /* stages of unpacked weights in tensor memory, 64 columns each */
 constexpr int kTcD = 4;        /* accumulators */
 constexpr int kTcWDepth = 6;   /* stages of a warp's weight ring */
 constexpr int kTcXDepth = 4;   /* stages of the vectors */
 constexpr int kTcHalf = kStageBlocks / 2;         /* blocks of a stage that an unpacking warp has */
 constexpr int kTcWStage = 32 * kTcHalf * 16;
 constexpr int kTcMaxSplit = 8;
+constexpr int kTcStreams = 64;
 
 struct TcShared {
-    uint64_t a_full[2], a_empty[2], x_full[kTcXDepth], x_empty[kTcXDepth], d_full[kTcD], d_empty[kTcD], drain;
+    uint64_t a_full[kTcA], a_empty[kTcA], x_full[kTcXDepth], x_empty[kTcXDepth], d_full[kTcD], d_empty[kTcD], drain;
     uint32_t tmem;
     int abort, never;
 };
@@ -734,6 +672,15 @@ template <int kCount> __device__ __forceinline__ void tc_load(uint32_t at, int (
         asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]) : : "memory");
 }
 
+/* A thread's results, n of kCount streams from b0, of a row. */
+template <typename T, int kCount>
+__device__ __forceinline__ void store_row(const MatvecParams &p, int b0, int n, int row, const float (&acc)[kCount]) {
+    T *y = (T *)p.y + (size_t)b0 * p.y_stride + row;
+#pragma unroll
+    for (int j = 0; j < kCount; ++j, y += p.y_stride)
+        if (j < n) *y = from_f32<T>(__fmul_rn(__ldg(p.sx + b0 + j), __fmul_rn(0.0625f, acc[j])));
+}
+
 /* The stages of a CTA in order: every tile's range of K. */
 struct TcWalk {
     int tile, st, n = 0;
@@ -781,7 +728,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
     const int per = st1 - st0, total = my_tiles * per;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) mbar_init(&sh.a_full[i], kTcUnpack), mbar_init(&sh.a_empty[i], 1);
+        for (int i = 0; i < kTcA; ++i) mbar_init(&sh.a_full[i], kTcUnpack), mbar_init(&sh.a_empty[i], 1);
         for (int i = 0; i < kTcXDepth; ++i)
             mbar_init(&sh.x_full[i], kTcLoad), mbar_init(&sh.x_empty[i], 1 + (kMin ? kTcEpi : 0));
         for (int i = 0; i < kTcD; ++i) mbar_init(&sh.d_full[i], 1), mbar_init(&sh.d_empty[i], kTcEpi);
@@ -789,7 +736,8 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
         sh.abort = sh.never = 0;
         mbar_fence_init();
     }
-    constexpr int kCols = 128 + kTcD * kN <= 256 ? 256 : 512;
+    constexpr int kCols = 512;
+    static_assert(64 * kTcA + kTcD * kN <= kCols, "tensor memory");
     if (warp == kTcIssue) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(kCols)
                      : "memory");
@@ -798,7 +746,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem, tmem_d = tmem + 128; /* two A operands of 64 columns, then the accumulators */
+    const uint32_t tmem = sh.tmem, tmem_d = tmem + 64 * kTcA; /* the A operands, then the accumulators */
 
     float acc[kMine]; /* of an epilogue thread */
 
@@ -841,8 +789,8 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
 #pragma unroll
             for (int i = 0; i < kTcHalf; ++i) v[i] = *(const uint4 *)(row + ((i ^ ((lane >> 1) & 3)) << 4));
             slot = slot + 1 == kTcWDepth ? 0 : slot + 1;
-            const int buf = it & 1;
-            if (it >= 2 && !tc_wait(&sh.a_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag)) {
+            const int buf = it % kTcA;
+            if (it >= kTcA && !tc_wait(&sh.a_empty[buf], ((it / kTcA) & 1) ^ 1, abort_flag)) {
                 *abort_flag = 1;
                 break;
             }
@@ -946,10 +894,11 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             }
             if (splits == 1 && at.st == st1 - 1) {
                 const int row = at.tile * 128 + quad * 32 + lane;
-                if (row < p.rows)
-#pragma unroll
-                    for (int j = 0; j < kMine; ++j)
-                        if (part * kMine + j < nx) store_y(p, b0 + part * kMine + j, row, 0.0625f * acc[j]);
+                if (row < p.rows) {
+                    if (p.dtype == LAL_TAIL_F32) store_row<float>(p, b0 + part * kMine, nx - part * kMine, row, acc);
+                    else if (p.dtype == LAL_TAIL_BF16) store_row<__nv_bfloat16>(p, b0 + part * kMine, nx - part * kMine, row, acc);
+                    else store_row<__half>(p, b0 + part * kMine, nx - part * kMine, row, acc);
+                }
             }
         }
         if (!ok) {
@@ -971,9 +920,9 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             const uint32_t x0 = tc_desc_low(smem_u32(xring));
             int xs = 0, xs_round = 0;
             for (int it = 0, d = 0; it < total && ok; ++it) {
-                const int buf = it & 1;
+                const int buf = it % kTcA;
                 if (!tc_wait(&sh.x_full[xs], xs_round & 1, abort_flag) ||
-                    !tc_wait(&sh.a_full[buf], (it >> 1) & 1, abort_flag)) {
+                    !tc_wait(&sh.a_full[buf], (it / kTcA) & 1, abort_flag)) {
                     *abort_flag = 1;
                     break;
                 }
@@ -1105,8 +1054,9 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
     }
 }
 
-template <int kN, int kGroup, bool kMin>
+template <int kGroup, bool kMin>
 cudaError_t launch_tc(const MatvecParams &p, int x_base, int chunks, int num_sms, cudaStream_t st) {
+    constexpr int kN = kTcStreams;
     const int tiles = (p.rows + 127) / 128, stages = (q4_blocks(p.cols) + kStageBlocks - 1) / kStageBlocks;
     /* CTAs of a tile: as many as leave each an SM and two stages */
     int splits = 1;
@@ -1129,22 +1079,279 @@ cudaError_t launch_tc(const MatvecParams &p, int x_base, int chunks, int num_sms
     return cudaLaunchKernelEx(&cfg, q4_tc_kernel<kN, kGroup, kMin>, p, splits, x_base);
 }
 
+/* ---- many streams: the same products, the vectors shared by a CTA ----
+ *
+ * A CTA of eight warps takes a range of rows, 32 a warp and tile, by up to 8
+ * kNT streams.  A warp's weights and scales go through a ring of its own, as
+ * above; the vectors' part of a stage is loaded once for all (a barrier a
+ * stage), so that a stage's 8 kNT vectors serve 256 rows.  A CTA's ring runs on
+ * over its tiles. */
+constexpr int kWideDepth = 4;
+constexpr int kWideMT = 2, kWideNT = 4;
+
+struct WideShape {
+    int range, height; /* rows of a CTA; of a warp and tile */
+};
+
+template <int kGroup, bool kMin> struct WideStage {
+    static constexpr int kMT = kWideMT, kNT = kWideNT;
+    static constexpr int kGroups = kStageBlocks * kQ4Block / kGroup;
+    static constexpr int kWarps = 16 / kMT, kThreads = 32 * kWarps, kRows = 16 * kMT; /* rows of a warp */
+    static constexpr int kA = kRows * 128, kScale = kRows * kGroups * 2;
+    static constexpr int kW = (kA + (kMin ? 2 : 1) * kScale + 127) / 128 * 128; /* of a warp */
+    static constexpr int kX = 8 * kNT * kStageBlocks * 32;
+    static constexpr int kSmem = kWideDepth * (kX + kWarps * kW);
+    static_assert(kSmem <= 227 * 1024, "one CTA an SM");
+};
+
 template <int kGroup, bool kMin>
-cudaError_t launch_tc_all(const MatvecParams &p, int num_sms, cudaStream_t st) {
-    /* whole chunks of 64 streams, then the smallest tile that has the rest */
-    const int whole = p.streams / 64, rest = p.streams % 64;
-    if (whole > 0) {
-        const cudaError_t e = launch_tc<64, kGroup, kMin>(p, 0, whole, num_sms, st);
-        if (e != cudaSuccess || rest == 0) return e;
+__global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecParams p, const WideShape h, int b0) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    using Stage = WideStage<kGroup, kMin>;
+    constexpr int kMT = kWideMT, kNT = kWideNT;
+    constexpr int kWarps = Stage::kWarps, kGroups = Stage::kGroups, kPer = kGroup / kQ4Block;
+    constexpr int kUnit = kPer < 2 ? 2 : kPer;        /* blocks between two readings of the scales */
+    constexpr int kUnitGroups = kUnit / kPer, kUnits = kStageBlocks / kUnit;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
+    const int nx = p.streams - b0; /* at most 8 kNT */
+    const int nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
+    const int stages = (nb + kStageBlocks - 1) / kStageBlocks; /* of a row */
+    const int first = blockIdx.x * h.range, end = min(p.rows, first + h.range), tile_rows = kWarps * h.height;
+    const int tiles = (end - first + tile_rows - 1) / tile_rows, total = tiles * stages;
+    const uint32_t x_ring = smem_u32(smem), w_ring = x_ring + kWideDepth * Stage::kX + warp * kWideDepth * Stage::kW;
+
+    /* ---- loads ---- */
+    const int w_r = lane >> 3, w_k = lane & 7;
+    const uint32_t w_to = w_ring + w_r * 128 + ((w_k ^ w_r) << 4);
+    const size_t w_step = (size_t)nb * 64;
+    const uint8_t *w_src = nullptr;
+    const int x_n = threadIdx.x >> 4, x_c = threadIdx.x & 15; /* kXRows vectors at a time */
+    constexpr int kXRows = Stage::kThreads / 16;
+    const uint32_t x_to = x_ring + x_n * 256 + ((x_c ^ (x_n & 7)) << 4);
+    const int8_t *const x_src = p.x + (size_t)(b0 + min(x_n, nx - 1)) * p.x_stride;
+    const size_t x_step = (size_t)kXRows * p.x_stride;
+    const bool x_aligned = (((uintptr_t)p.x | (uintptr_t)p.x_stride) & 15) == 0;
+    const bool s_aligned =
+        (((uintptr_t)p.scale | (kMin ? (uintptr_t)p.min : 0) | (uintptr_t)(groups * 2)) & (2 * kGroups - 1)) == 0;
+    size_t s_row = 0;
+    int l_row = first + warp * h.height, l_st = 0, l_slot = 0, l_left = total, l_rows = 0;
+    auto load = [&] {
+        if (l_left > 0) {
+            if (l_st == 0) { /* a tile begins */
+                l_rows = min(h.height, end - l_row); /* may be below 1 */
+                w_src = p.q + ((size_t)(l_row + w_r) * nb + w_k) * 16;
+                s_row = (size_t)(l_row + lane) * groups;
+                l_row += tile_rows;
+            }
+            const int k0 = l_st * kStageBlocks;
+            const uint32_t base = l_slot * Stage::kW;
+            if (k0 + w_k < nb) {
+#pragma unroll
+                for (int j = 0; j < 4 * kMT; ++j)
+                    if (w_r + 4 * j < l_rows) cp_async16((w_to + base + j * 512) ^ (j & 1 ? 64 : 0), w_src + j * w_step, 16);
+            }
+            w_src += kStageBlocks * 16;
+            const int c0 = k0 * kQ4Block + x_c * 16;
+            const uint32_t to = x_to + l_slot * Stage::kX;
+            if (x_aligned && c0 + 16 <= p.cols) {
+                const int8_t *x = x_src + c0;
+#pragma unroll
+                for (int j = 0; j < (8 * kNT + kXRows - 1) / kXRows; ++j, x += x_step)
+                    if (x_n + kXRows * j < nx) cp_async16_l1(to + j * (kXRows * 256), x, 16);
+            } else {
+                const int8_t *x = x_src;
+#pragma unroll 1
+                for (int j = 0; x_n + kXRows * j < nx; ++j, x += x_step)
+                    stage_x16(smem + (to - x_ring) + j * (kXRows * 256), x, c0, p.cols, x_aligned);
+            }
+            if (lane < l_rows) {
+                const int g0 = l_st * kGroups;
+#pragma unroll
+                for (int m = 0; m < (kMin ? 2 : 1); ++m) {
+                    const unsigned short *src = (const unsigned short *)(m ? p.min : p.scale) + s_row + g0;
+                    const uint32_t dst = w_ring + base + Stage::kA + m * Stage::kScale + lane * (2 * kGroups);
+                    if (s_aligned && g0 + kGroups <= groups) {
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(2 * kGroups) : "memory");
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < kGroups; ++k) {
+                            const unsigned short v = g0 + k < groups ? __ldg(src + k) : 0;
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + 2 * k), "h"(v) : "memory");
+                        }
+                    }
+                }
+            }
+            --l_left;
+            if (++l_slot == kWideDepth) l_slot = 0;
+            if (++l_st == stages) l_st = 0;
+        }
+        cp_async_commit();
+    };
+    for (int i = 0; i < kWideDepth - 1; ++i) load();
+
+    /* ---- products ---- */
+    const uint32_t a_at = w_ring + (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+    const uint32_t x_at = x_ring + (lane & 7) * 256 + (((lane >> 3) ^ (lane & 7)) << 4);
+    const uint32_t s_at = w_ring + Stage::kA + g * (2 * kGroups);
+    float acc[kMT][kNT][4];
+    int slot = 0, st = 0, row0 = first + warp * h.height;
+    for (int it = 0; it < total; ++it) {
+        cp_async_wait<kWideDepth - 2>();
+        __syncthreads();
+        load();
+        if (st == 0)
+#pragma unroll
+            for (int m = 0; m < kMT; ++m)
+#pragma unroll
+                for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
+        if (row0 < end) {
+            /* blocks behind the row's end hold zeros in the vectors, and their groups scales of zero */
+            const uint32_t at = slot * Stage::kW, xt = slot * Stage::kX;
+#pragma unroll(kNT <= 2 ? kUnits : 1)
+            for (int u = 0; u < kUnits; ++u) {
+                uint32_t a[kMT][kUnit][4];
+#pragma unroll
+                for (int m = 0; m < kMT; ++m)
+#pragma unroll
+                    for (int q = 0; q < kUnit / 2; ++q) {
+                        uint32_t w[4];
+                        ldmatrix4(w, (a_at + at + m * 2048) ^ ((u * (kUnit / 2) + q) << 5));
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            a[m][2 * q + k][0] = ((w[2 * k] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+                            a[m][2 * q + k][1] = ((w[2 * k + 1] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+                            a[m][2 * q + k][2] = (w[2 * k] & 0xf0f0f0f0u) ^ 0x80808080u;
+                            a[m][2 * q + k][3] = (w[2 * k + 1] & 0xf0f0f0f0u) ^ 0x80808080u;
+                        }
+                    }
+                float s[kMT][2][kUnitGroups], l[kMT][2][kUnitGroups];
+#pragma unroll
+                for (int m = 0; m < kMT; ++m)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const uint32_t from = s_at + at + (16 * m + 8 * r) * (2 * kGroups) + u * (2 * kUnitGroups);
+                        uint32_t v, w = 0;
+                        if (kUnitGroups == 2) {
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+                            if (kMin) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from + Stage::kScale) : "memory");
+                        } else {
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+                            if (kMin) asm volatile("ld.shared.u16 %0, [%1];" : "=r"(w) : "r"(from + Stage::kScale) : "memory");
+                        }
+#pragma unroll
+                        for (int k = 0; k < kUnitGroups; ++k) {
+                            s[m][r][k] = __half2float(__ushort_as_half((unsigned short)(v >> (16 * k))));
+                            if (kMin)
+                                l[m][r][k] = fmaf(8.0f, s[m][r][k], __half2float(__ushort_as_half((unsigned short)(w >> (16 * k)))));
+                        }
+                    }
+                /* kB eights of vectors at once: as many independent products again */
+                constexpr int kB = kNT < 2 ? 1 : 2;
+#pragma unroll
+                for (int n0 = 0; n0 < kNT; n0 += kB) {
+                    uint32_t x[kB][kUnit / 2][4];
+#pragma unroll
+                    for (int n = 0; n < kB; ++n)
+#pragma unroll
+                        for (int q = 0; q < kUnit / 2; ++q) {
+                            const int pair = u * (kUnit / 2) + q;
+                            ldmatrix4(x[n][q], ((x_at + xt + (n0 + n) * 2048) ^ ((pair & 1) << 6)) + (pair >> 1) * 128);
+                        }
+#pragma unroll
+                    for (int k = 0; k < kUnitGroups; ++k) {
+                        int c[kB][kMT][4], cx[kB][4];
+#pragma unroll
+                        for (int j = 0; j < kPer; ++j) {
+                            const int i = k * kPer + j;
+#pragma unroll
+                            for (int n = 0; n < kB; ++n) {
+                                const uint32_t x0 = x[n][i / 2][2 * (i % 2)], x1 = x[n][i / 2][2 * (i % 2) + 1];
+                                if (kMin) {
+                                    const uint32_t ones[4] = {0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u};
+                                    if (j == 0) mma_s8_zero(cx[n], ones, x0, x1);
+                                    else mma_s8(cx[n], ones, x0, x1);
+                                }
+#pragma unroll
+                                for (int m = 0; m < kMT; ++m) {
+                                    if (j == 0) mma_s8_zero(c[n][m], a[m][i], x0, x1);
+                                    else mma_s8(c[n][m], a[m][i], x0, x1);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int n = 0; n < kB; ++n)
+#pragma unroll
+                            for (int m = 0; m < kMT; ++m)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    float &to = acc[m][n0 + n][i];
+                                    to = fmaf(s[m][i >> 1][k], (float)c[n][m][i], to);
+                                    if (kMin) to = fmaf(l[m][i >> 1][k], (float)cx[n][i & 1], to);
+                                }
+                    }
+                }
+            }
+        }
+        if (++slot == kWideDepth) slot = 0;
+        if (++st < stages) continue;
+        st = 0;
+        store_tile(p, b0, nx, row0, min(h.height, end - row0), acc);
+        row0 += tile_rows;
     }
-    return rest <= 16   ? launch_tc<16, kGroup, kMin>(p, whole * 64, 1, num_sms, st)
-           : rest <= 32 ? launch_tc<32, kGroup, kMin>(p, whole * 64, 1, num_sms, st)
-                        : launch_tc<64, kGroup, kMin>(p, whole * 64, 1, num_sms, st);
+    cp_async_wait<0>();
+}
+
+template <int kGroup, bool kMin>
+cudaError_t launch_wide(const MatvecParams &p, int x_base, int num_sms, cudaStream_t st) {
+    /* equal ranges of rows, so that every SM reads as much; tiles as equal as they go */
+    using Stage = WideStage<kGroup, kMin>;
+    constexpr int kTile = Stage::kRows * Stage::kWarps;
+    WideShape h;
+    h.range = std::max((p.rows + num_sms - 1) / num_sms, std::min(p.rows, kTile / 2));
+    const int n = (h.range + kTile - 1) / kTile;
+    h.height = (h.range + n * Stage::kWarps - 1) / (n * Stage::kWarps);
+    const cudaError_t e = raise_smem((const void *)q4_wide_kernel<kGroup, kMin>, Stage::kSmem);
+    if (e != cudaSuccess) return e;
+    q4_wide_kernel<kGroup, kMin><<<(p.rows + h.range - 1) / h.range, Stage::kThreads, Stage::kSmem, st>>>(p, h, x_base);
+    return cudaGetLastError();
+}
+
+/* Which kernel.  Measured on a B200, us:
+ *   streams  weights            mma    shared vectors  tcgen05
+ *   8        152064x3584 g128   56     58              123
+ *   16       37888x3584  g32    24.1   22.1            55
+ *   32       37888x3584  g128   31.4   22.8            33.7
+ *   32       3584x18944  g32    33.0   23.6            45.7
+ *   32       3584x3584   g32    11.5   14.4            15.4
+ *   64       37888x3584  g128   61     43.4            36.2
+ *   64       3584x18944  g128   45     35.4            29.5
+ * so mma up to 16 streams, shared vectors up to 32 where the weights are
+ * many, tcgen05 beyond, in chunks of 64 streams and the rest. */
+template <int kGroup, bool kMin>
+cudaError_t launch_streams(const MatvecParams &p, int x_base, int num_sms, cudaStream_t st) {
+    const int n = p.streams - x_base;
+    const long long weights = (long long)p.rows * p.cols;
+    if (n > 32) return launch_tc<kGroup, kMin>(p, x_base, 1, num_sms, st);
+    if (n > 16 && weights >= (long long)num_sms * 256 * 1024) return launch_wide<kGroup, kMin>(p, x_base, num_sms, st);
+    if (n > 8)
+        return (p.rows + 31) / 32 >= 2 * num_sms * mma_warps(true) ? launch_mma<2, 2, kGroup, kMin, true>(p, x_base, num_sms, st)
+                                                                   : launch_mma<2, 2, kGroup, kMin, false>(p, x_base, num_sms, st);
+    /* 32 rows a warp share its part of the vectors: fewer instructions, but half the warps.  Eight
+     * streams, groups of 32: 16.3 us against 20.0 for 37888x3584, 6.2 against 5.8 for 5000x1000; groups
+     * of 128, where the instructions do not bound: 61 against 57 for 152064x3584. */
+    if (kGroup == 32 && weights >= (long long)num_sms * 256 * 1024) return launch_mma<2, 1, kGroup, kMin, false>(p, x_base, num_sms, st);
+    return launch_mma<1, 1, kGroup, kMin, false>(p, x_base, num_sms, st);
 }
 
 template <int kGroup, bool kMin> cudaError_t launch_matvec(const MatvecParams &p, int num_sms, cudaStream_t st) {
-    if (p.streams > kMmaStreams) return launch_tc_all<kGroup, kMin>(p, num_sms, st);
-    return p.streams <= 3 ? launch_mma<kGroup, kMin, 4>(p, num_sms, st) : launch_mma<kGroup, kMin, 3>(p, num_sms, st);
+    const int whole = p.streams / kTcStreams;
+    if (whole > 0) {
+        const cudaError_t e = launch_tc<kGroup, kMin>(p, 0, whole, num_sms, st);
+        if (e != cudaSuccess || whole * kTcStreams == p.streams) return e;
+    }
+    return launch_streams<kGroup, kMin>(p, whole * kTcStreams, num_sms, st);
 }
 
 template <int kGroup> cudaError_t launch_matvec(const MatvecParams &p, int num_sms, cudaStream_t st) {
@@ -1262,7 +1469,6 @@ int lal_tail_q4_matvec(const lal_tail_q4 *w, const int8_t *d_xq, int64_t xq_stri
                             (const __half *)w->d_min, n_streams, w->rows, w->cols, w->group, d_y, y_stride, dtype};
     cudaStream_t st = (cudaStream_t)stream;
     const int sms = dev.num_sms();
-    if (n_streams == 1 && dot_smem(p, n_streams) >= 0) return launched(op, launch_dot<1>(p, sms, st));
     return launched(op, w->group == 32   ? launch_matvec<32>(p, sms, st)
                         : w->group == 64 ? launch_matvec<64>(p, sms, st)
                                          : launch_matvec<128>(p, sms, st));
