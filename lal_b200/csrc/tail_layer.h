@@ -118,6 +118,16 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
     return __float2bfloat16_rn(v);
 }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+/* two 16-bit numbers of a word */
+template <typename T> __device__ __forceinline__ void unpack16(uint32_t w, float &a, float &b);
+template <> __device__ __forceinline__ void unpack16<__nv_bfloat16>(uint32_t w, float &a, float &b) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xffff0000u);
+}
+template <> __device__ __forceinline__ void unpack16<__half>(uint32_t w, float &a, float &b) {
+    a = __half2float(__ushort_as_half((unsigned short)w));
+    b = __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+}
 #endif
 
 }  // namespace lal

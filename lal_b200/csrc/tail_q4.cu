@@ -27,17 +27,32 @@ __host__ __device__ inline int q4_blocks(int cols) { return (cols + kQ4Block - 1
 
 /* ---------------------------------------------------------- quantizer --- */
 
-/* rint((w - m) / s) of the quotient in 64 bits: 32 bits where they cannot be
- * on the wrong side of a border (the quotient is below 16, and three roundings
- * of 2^-24 each are below 3e-6) */
-__device__ __noinline__ int q4_round64(float w, float m, float s) {
-    return (int)rint(((double)w - (double)m) / (double)s);
+/* rint((w - m) / s) exactly, ties to even, from n that is off by one at most:
+ * w - m as the sum of two fp32 numbers, less n s (11 and 4 bits: exact), against
+ * half a step.  Near half a step the difference has no more than 24 bits. */
+__device__ __forceinline__ float q4_exact(float w, float m, float s, float n) {
+    const float d = __fsub_rn(w, m), bb = __fsub_rn(d, w);
+    const float low = __fadd_rn(__fsub_rn(w, __fsub_rn(d, bb)), -__fadd_rn(m, bb));
+    const float e = fmaf(-n, s, d), half = __fmul_rn(0.5f, s);
+    const float over = __fadd_rn(__fsub_rn(e, half), low), under = __fadd_rn(__fadd_rn(e, half), low);
+    const bool odd = (__float2int_rn(n) & 1) != 0;
+    if (over > 0.0f || (over == 0.0f && odd)) n += 1.0f;
+    if (under < 0.0f || (under == 0.0f && odd)) n -= 1.0f;
+    return n;
 }
-__device__ __forceinline__ int q4_round(float w, float m, float s, float r) {
-    const float t = __fmul_rn(__fsub_rn(w, m), r);
-    const float n = rintf(t);
-    if (fabsf(t - n) < 0.5f - 4e-6f) return (int)n;
-    return q4_round64(w, m, s);
+
+/* The smallest f16 s with k s >= x: rounded up, so no weight is clamped.  k s is
+ * an fp32 number (11 and 4 bits), so it compares exactly; the nearest f16 to
+ * x / k is s or one step below.  Infinite above f16's range. */
+__device__ __forceinline__ __half f16_step_up(float x, float k, float k_inv) {
+    const __half h = __float2half_rn(__fmul_rn(x, k_inv));
+    return __fmul_rn(k, __half2float(h)) < x ? __ushort_as_half((unsigned short)(__half_as_ushort(h) + 1)) : h;
+}
+/* the largest f16 not above x */
+__device__ __forceinline__ __half f16_floor(float x) {
+    const __half h = __float2half_rn(x);
+    const unsigned short b = __half_as_ushort(h);
+    return __half2float(h) > x ? __ushort_as_half((unsigned short)(b & 0x8000 ? b + 1 : b - 1)) : h;
 }
 
 /* Four elements from p on, of which n (may be below 0) exist. */
@@ -47,14 +62,9 @@ template <typename T> __device__ __forceinline__ void get4(const T *p, int n, bo
             const float4 f = __ldg((const float4 *)p);
             v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
         } else {
-            union Raw {
-                uint2 w;
-                T e[4];
-                __device__ Raw() {}
-            } raw;
-            raw.w = __ldg((const uint2 *)p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = to_f32(raw.e[i]);
+            const uint2 w = __ldg((const uint2 *)p);
+            unpack16<T>(w.x, v[0], v[1]);
+            unpack16<T>(w.y, v[2], v[3]);
         }
     } else {
 #pragma unroll
@@ -82,9 +92,17 @@ template <typename T> __device__ __forceinline__ void put4(T *p, int n, bool ali
     }
 }
 
-/* Both directions: a lane takes a 32-bit word, columns 4u .. 4u + 3 and 16 +
- * 4u .. of a block; a warp takes kRun runs of 256 columns of a row, all their
- * loads at once. */
+/* Four elements as they lie in memory. */
+template <typename T> union Four {
+    uint32_t w[sizeof(T)];
+    T e[4];
+    __device__ Four() {}
+};
+
+/* Both directions: four lanes a block, a warp takes kRun runs of 256 columns of
+ * a row, all their loads at once.  Of fp32, lane u of a block has columns 4u ..
+ * 4u + 3 and 16 + 4u .., which are the word u; of 16-bit numbers eight columns
+ * in a row, 16 bytes, and half a word's worth goes over to another lane. */
 constexpr int kRun = 4;
 constexpr int kQ4Warps = 8;
 struct ConvertParams {
@@ -93,52 +111,67 @@ struct ConvertParams {
     int rows, cols, group;
     void *w;
     long long w_stride;
-    int aligned; /* rows of w are aligned to four elements */
+    int aligned; /* rows of w are aligned to 16 bytes */
 };
-inline long long q4_runs(int rows, int cols) { return (long long)rows * ((cols + 255) / 256); }
-inline unsigned q4_ctas(int rows, int cols) {
-    return (unsigned)((q4_runs(rows, cols) + kRun * kQ4Warps - 1) / (kRun * kQ4Warps));
-}
+/* warps: kRun * 256 columns of a row each */
+__host__ __device__ inline int q4_row_warps(int cols) { return (cols + kRun * 256 - 1) / (kRun * 256); }
+inline long long q4_ctas(int rows, int cols) { return ((long long)rows * q4_row_warps(cols) + kQ4Warps - 1) / kQ4Warps; }
 
 template <typename T, int kGroup, bool kMin>
 __global__ void __launch_bounds__(32 * kQ4Warps) quantize_q4_kernel(const ConvertParams p) {
     const int lane = threadIdx.x & 31, nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
-    const int per_row = (p.cols + 255) / 256;
-    const long long run0 = ((long long)blockIdx.x * kQ4Warps + (threadIdx.x >> 5)) * kRun;
+    constexpr bool kRow8 = sizeof(T) == 2;
+    const int per_row = q4_row_warps(p.cols);
+    const long long at = (long long)blockIdx.x * kQ4Warps + (threadIdx.x >> 5);
+    const int row = (int)(at / per_row), c0 = (int)(at - (long long)row * per_row) * (kRun * 256);
+    if (row >= p.rows) return;
     float v[kRun][8];
-    int row = (int)(run0 / per_row), seg = (int)(run0 - (long long)row * per_row);
-    const int row_0 = row, seg_0 = seg;
-    auto step = [&] {
-        if (++seg == per_row) seg = 0, ++row;
-    };
+    const T *const w0 = (const T *)p.w + (size_t)row * p.w_stride + c0 + (lane >> 2) * 32 + (lane & 3) * (kRow8 ? 8 : 4);
 #pragma unroll
-    for (int u = 0; u < kRun; ++u, step()) {
-        if (row >= p.rows) break;
-        const int c = seg * 256 + (lane >> 2) * 32 + (lane & 3) * 4;
-        const T *w = (const T *)p.w + (size_t)row * p.w_stride + c;
+    for (int u = 0; u < kRun; ++u) {
+        if (c0 + u * 256 >= p.cols) break;
+        const int c = c0 + u * 256 + (lane >> 2) * 32 + (lane & 3) * (kRow8 ? 8 : 4);
+        const T *w = w0 + u * 256;
         float lo[4], hi[4];
-        get4(w, p.cols - c, p.aligned, lo);
-        get4(w + 16, p.cols - c - 16, p.aligned, hi);
+        if constexpr (kRow8) {
+            if (p.aligned && c + 8 <= p.cols) {
+                const uint4 x = __ldg((const uint4 *)w);
+                unpack16<T>(x.x, lo[0], lo[1]);
+                unpack16<T>(x.y, lo[2], lo[3]);
+                unpack16<T>(x.z, hi[0], hi[1]);
+                unpack16<T>(x.w, hi[2], hi[3]);
+            } else {
+                get4(w, p.cols - c, false, lo);
+                get4(w + 4, p.cols - c - 4, false, hi);
+            }
+        } else {
+            get4(w, p.cols - c, p.aligned, lo);
+            get4(w + 16, p.cols - c - 16, p.aligned, hi);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[u][i] = lo[i], v[u][4 + i] = hi[i];
     }
-    row = row_0, seg = seg_0;
+    uint32_t *const q0 = (uint32_t *)p.q + ((size_t)row * nb + c0 / kQ4Block + (lane >> 2)) * 4;
+    const size_t s0 = (size_t)row * groups;
 #pragma unroll
-    for (int u = 0; u < kRun; ++u, step()) {
-        if (row >= p.rows) break;
-        const int c = seg * 256 + (lane >> 2) * 32 + (lane & 3) * 4;
-        /* what does not exist is 0 to the absolute largest, and left out of the extremes */
-        float hi = -INFINITY, lo = INFINITY, top = 0.0f;
-        bool bad = false;
+    for (int u = 0; u < kRun; ++u) {
+        if (c0 + u * 256 >= p.cols) break;
+        const int c = c0 + u * 256 + (lane >> 2) * 32; /* the block's first column */
+        /* max|w|, NaN above all; what does not exist is 0 to it, and left out of the extremes */
+        float top = 0.0f, hi = -INFINITY, lo = INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bool in = c + (i < 4 ? i : 12 + i) < p.cols;
-            const float a = fabsf(v[u][i]);
-            bad |= !(a <= 3.4028234663852886e38f);
-            top = fmaxf(top, a);
-            if (kMin && in) hi = fmaxf(hi, v[u][i]), lo = fminf(lo, v[u][i]);
+        for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(v[u][i])));
+        if (kMin) {
+            if (c0 + u * 256 + 256 <= p.cols) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) hi = fmaxf(hi, v[u][i]), lo = fminf(lo, v[u][i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (c + (kRow8 ? (lane & 3) * 8 + i : (lane & 3) * 4 + (i < 4 ? i : 12 + i)) < p.cols) hi = fmaxf(hi, v[u][i]), lo = fminf(lo, v[u][i]);
+            }
         }
-        int worst = bad ? 0x7f800000 : __float_as_int(top);
+        unsigned worst = __float_as_uint(top) & 0x7fffffffu;
 #pragma unroll
         for (int o = kGroup / 16; o > 0; o >>= 1) { /* 4 lanes a block */
             worst = max(worst, __shfl_xor_sync(0xffffffffu, worst, o));
@@ -147,37 +180,55 @@ __global__ void __launch_bounds__(32 * kQ4Warps) quantize_q4_kernel(const Conver
                 lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
             }
         }
-        bad = worst >= 0x7f800000;
-        /* Rounded outwards step by step, which is rounding outwards once: f16
-         * numbers and their multiples by 7 or 15 are fp32 numbers too. */
         __half s, m = __float2half_rn(0.0f);
         if (kMin) {
-            m = __float2half_rd(lo);
-            s = __float2half_ru(__fdiv_ru(__fsub_ru(hi, __half2float(m)), 15.0f));
-            bad |= __hisinf(m) != 0;
+            m = f16_floor(lo);
+            s = f16_step_up(__fsub_ru(hi, __half2float(m)), 15.0f, 1.0f / 15.0f);
         } else {
-            s = __float2half_ru(__fdiv_ru(__int_as_float(worst), 7.0f));
+            s = f16_step_up(__uint_as_float(worst), 7.0f, 1.0f / 7.0f);
         }
-        bad |= __hisinf(s) != 0;
+        const bool bad = worst >= 0x7f800000u || __hisinf(s) != 0 || (kMin && __hisinf(m) != 0);
         const float sf = __half2float(s), mf = __half2float(m);
-        const bool some = !bad && sf > 0.0f;
-        const float r = some ? __frcp_rn(sf) : 0.0f;
-        uint32_t word = 0;
+        uint32_t low = 0, high = 0;
+        if (!bad && sf > 0.0f) {
+            float r, far = 0.0f;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(sf));
+            constexpr float kRound = 12582912.0f; /* 1.5 * 2^23: added, it leaves the nearest integer in the low bits */
+            uint32_t n[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            int q = kMin ? 0 : 8;
-            if (some) {
-                const int n = q4_round(v[u][i], mf, sf, r);
-                q = kMin ? max(0, min(15, n)) : max(-7, min(7, n)) + 8;
+            for (int i = 0; i < 8; ++i) {
+                float t = __fmul_rn(kMin ? __fsub_rn(v[u][i], mf) : v[u][i], r);
+                /* 11 bits by 11: the quotient is halfway between two steps, and then this is it, or 2^-12 away */
+                if (kRow8 && !kMin) t = fmaf(fmaf(-t, sf, v[u][i]), r, t);
+                const float x = __fadd_rn(t, kRound);
+                if (!kRow8 || kMin) far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(x, kRound))));
+                n[i] = __float_as_uint(x);
             }
-            word |= (uint32_t)q << (i < 4 ? 8 * i : 8 * (i - 4) + 4);
+            /* three roundings of a quotient below 16, 2^-22 of it together: below 4e-6 */
+            if (!(far < 0.5f - 8e-6f))
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    n[i] = __float_as_uint(__fadd_rn(
+                        q4_exact(v[u][i], mf, sf, __fsub_rn(__uint_as_float(n[i]), kRound)), kRound));
+            low = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+            high = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
         }
+        int place = lane & 3;
+        if (kRow8) {
+            /* lanes 0 and 1 have columns 0-15, a word's low halves; 2 and 3 the high ones: lanes 0, 2, 1, 3 end with words 0, 1, 2, 3 */
+            const bool first = place < 2;
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, first ? high : low, 2);
+            (first ? high : low) = got;
+            place = (place & 1) * 2 + (place >> 1);
+        }
+        /* -7 .. 7, plus 8: the sign bit of four turned */
+        const uint32_t word = ((low & 0x0f0f0f0fu) | ((high << 4) & 0xf0f0f0f0u)) ^ (kMin ? 0u : 0x88888888u);
         if (c / kQ4Block < nb) {
-            ((uint32_t *)p.q)[((size_t)row * nb + c / kQ4Block) * 4 + (lane & 3)] = word;
-            if (c % kGroup == 0) {
+            q0[u * 32 + place] = word;
+            if ((lane & 3) == 0 && c % kGroup == 0) {
                 const __half nan = __ushort_as_half(0x7e00);
-                p.scale[(size_t)row * groups + c / kGroup] = bad ? nan : s;
-                if (kMin) p.min[(size_t)row * groups + c / kGroup] = bad ? nan : m;
+                p.scale[s0 + c / kGroup] = bad ? nan : s;
+                if (kMin) p.min[s0 + c / kGroup] = bad ? nan : m;
             }
         }
     }
@@ -186,41 +237,66 @@ __global__ void __launch_bounds__(32 * kQ4Warps) quantize_q4_kernel(const Conver
 template <typename T, int kGroup, bool kMin>
 __global__ void __launch_bounds__(32 * kQ4Warps) dequantize_q4_kernel(const ConvertParams p) {
     const int lane = threadIdx.x & 31, nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
-    const int per_row = (p.cols + 255) / 256;
-    const long long run0 = ((long long)blockIdx.x * kQ4Warps + (threadIdx.x >> 5)) * kRun;
-    int row = (int)(run0 / per_row), seg = (int)(run0 - (long long)row * per_row);
-    const int row_0 = row, seg_0 = seg;
-    auto step = [&] {
-        if (++seg == per_row) seg = 0, ++row;
-    };
+    const int per_row = q4_row_warps(p.cols);
+    const long long at = (long long)blockIdx.x * kQ4Warps + (threadIdx.x >> 5);
+    const int row = (int)(at / per_row), c0 = (int)(at - (long long)row * per_row) * (kRun * 256);
+    if (row >= p.rows) return;
+    const uint32_t *const q0 = (const uint32_t *)p.q + ((size_t)row * nb + c0 / kQ4Block) * 4 + lane;
+    const size_t s0 = (size_t)row * groups;
+    __shared__ __align__(16) T lines[kQ4Warps][256]; /* for rows that are not aligned */
+    T *const line = lines[threadIdx.x >> 5];
     uint32_t word[kRun];
     float s[kRun], m[kRun];
 #pragma unroll
-    for (int u = 0; u < kRun; ++u, step()) {
-        const int c = seg * 256 + (lane >> 2) * 32;
-        if (row >= p.rows) break;
+    for (int u = 0; u < kRun; ++u) {
+        const int c = c0 + u * 256 + (lane >> 2) * 32;
+        word[u] = 0;
         if (c >= p.cols) continue;
-        word[u] = __ldg((const uint32_t *)p.q + ((size_t)row * nb + c / kQ4Block) * 4 + (lane & 3));
-        s[u] = __half2float(p.scale[(size_t)row * groups + c / kGroup]);
-        m[u] = kMin ? __half2float(p.min[(size_t)row * groups + c / kGroup]) : 0.0f;
+        word[u] = __ldg(q0 + u * 32);
+        s[u] = __half2float(p.scale[s0 + c / kGroup]);
+        m[u] = kMin ? __half2float(p.min[s0 + c / kGroup]) : 0.0f;
     }
-    row = row_0, seg = seg_0;
+    T *const w0 = (T *)p.w + (size_t)row * p.w_stride + c0;
 #pragma unroll
-    for (int u = 0; u < kRun; ++u, step()) {
-        const int c = seg * 256 + (lane >> 2) * 32 + (lane & 3) * 4;
-        if (row >= p.rows) break;
-        if (c >= p.cols) continue;
-        T *w = (T *)p.w + (size_t)row * p.w_stride + c;
+    for (int u = 0; u < kRun; ++u) {
+        const int c = (lane >> 2) * 32 + (lane & 3) * 4, left = p.cols - c0 - u * 256;
+        if (left <= 0) break;
+        T *const w = w0 + u * 256;
+        float v[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float v[4];
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float q = (float)((word[u] >> (8 * i + 4 * h)) & 15u);
                 /* s * q is exact in 32 bits (11 and 4 bits): one rounding */
-                v[i] = kMin ? fmaf(s[u], q, m[u]) : __fmul_rn(s[u], q - 8.0f);
+                v[h][i] = kMin ? fmaf(s[u], q, m[u]) : __fmul_rn(s[u], q - 8.0f);
             }
-            put4(w + 16 * h, p.cols - c - 16 * h, p.aligned, v);
+        if (sizeof(T) == 2 && p.aligned && left >= 256) {
+            /* an even lane gives its high columns and takes its neighbour's low ones: eight in a row, 16 bytes */
+            Four<T> own[2], got;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) own[h].e[i] = from_f32<T>(v[h][i]);
+            const bool h = (lane & 1) != 0;
+            got.w[0] = __shfl_xor_sync(0xffffffffu, h ? own[0].w[0] : own[1].w[0], 1);
+            got.w[1] = __shfl_xor_sync(0xffffffffu, h ? own[0].w[1] : own[1].w[1], 1);
+            const uint4 x = h ? make_uint4(got.w[0], got.w[1], own[1].w[0], own[1].w[1])
+                              : make_uint4(own[0].w[0], own[0].w[1], got.w[0], got.w[1]);
+            *(uint4 *)(w + (lane >> 2) * 32 + (lane & 1) * 16 + (lane & 2) * 4) = x;
+            continue;
+        }
+        if (!p.aligned) __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (p.aligned) put4(w + c + 16 * h, left - c - 16 * h, true, v[h]);
+            else put4(line + c + 16 * h, 4, true, v[h]);
+        }
+        if (!p.aligned) { /* consecutive lanes, consecutive elements */
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 256; i += 32)
+                if (i + lane < left) w[i + lane] = line[i + lane];
         }
     }
 }
@@ -1361,7 +1437,7 @@ template <int kGroup> cudaError_t launch_matvec(const MatvecParams &p, int num_s
 /* one of the conversions' kernels by type, group and minimum */
 template <typename T, int kGroup>
 cudaError_t launch_convert(const ConvertParams &p, bool back, cudaStream_t st) {
-    const unsigned n = q4_ctas(p.rows, p.cols);
+    const unsigned n = (unsigned)q4_ctas(p.rows, p.cols);
     if (back && p.min) dequantize_q4_kernel<T, kGroup, true><<<n, 32 * kQ4Warps, 0, st>>>(p);
     else if (back) dequantize_q4_kernel<T, kGroup, false><<<n, 32 * kQ4Warps, 0, st>>>(p);
     else if (p.min) quantize_q4_kernel<T, kGroup, true><<<n, 32 * kQ4Warps, 0, st>>>(p);
@@ -1413,14 +1489,14 @@ int convert_q4(const char *op, const lal_tail_q4 *w, void *d_w, int64_t w_stride
     const WeightSpans spans(w);
     if (spans.meets(Span(d_w, w->rows, w->cols, w_stride, size)) || spans.meet_each_other())
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: buffers overlap", op);
-    if (q4_runs(w->rows, w->cols) / (kRun * kQ4Warps) >= 0x7fffffffLL)
+    if (q4_ctas(w->rows, w->cols) > 0x7fffffffLL)
         return layer_fail(LAL_TAIL_ERR_UNSUPPORTED, "%s: weights of %d x %d", op, w->rows, w->cols);
     static const char *const names[] = {"d_w", "d_q", "d_scale", "d_min"};
     const void *ptrs[] = {d_w, w->d_q, w->d_scale, w->d_min};
     CallDevice dev;
     if (const int rc = dev.enter(op, names, ptrs, 4)) return rc;
     const ConvertParams p = {w->d_q, (__half *)w->d_scale, (__half *)w->d_min, w->rows, w->cols, w->group, d_w, w_stride,
-                             ((uintptr_t)d_w | (uintptr_t)w_stride * size) % (4 * size) == 0};
+                             ((uintptr_t)d_w | (uintptr_t)w_stride * size) % 16 == 0};
     cudaStream_t st = (cudaStream_t)stream;
     return launched(op, dtype == LAL_TAIL_F32    ? launch_convert<float>(p, back, st)
                         : dtype == LAL_TAIL_BF16 ? launch_convert<__nv_bfloat16>(p, back, st)
