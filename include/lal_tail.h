@@ -378,7 +378,8 @@ int lal_tail_debug_expf(const float *x, float *y, int n);
  * beyond their type's.  Each call enqueues its work on `stream` (a
  * cudaStream_t of that device; NULL = its legacy default stream) and returns;
  * it allocates nothing, keeps nothing, shares no workspace, and can be
- * captured.  Zero rows or streams: nothing is done.  Only the rows and columns
+ * captured.  Zero rows or streams: nothing is done; rows and columns go up to
+ * 2^30 (rows of the 8-bit operators up to 2^31 - 1).  Only the rows and columns
  * named are written, and no output may overlap another buffer of the call,
  * except where a call says so.  A row's results do not depend on what the
  * other rows or streams of a call hold, and are the same in every run. */

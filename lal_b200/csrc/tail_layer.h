@@ -26,6 +26,9 @@ inline int layer_fail(int code, const char *fmt, ...) {
     return set_error(code, buf);
 }
 
+/* Rows and columns of a call: indexes rounded up to a tile stay within int. */
+constexpr int kLayerMaxDim = 1 << 30;
+
 inline int dtype_size(int dtype) {
     return dtype == LAL_TAIL_F32 ? 4 : dtype == LAL_TAIL_BF16 || dtype == LAL_TAIL_F16 ? 2 : 0;
 }

@@ -1454,7 +1454,7 @@ int check_weights(const char *op, const lal_tail_q4 *w) {
     if (!w) return layer_fail(LAL_TAIL_ERR_ARG, "%s: null weights", op);
     if (w->group != 32 && w->group != 64 && w->group != 128)
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: groups of %d columns (32, 64 or 128)", op, w->group);
-    if (w->rows < 0 || w->cols < 1)
+    if (w->rows < 0 || w->cols < 1 || w->rows > kLayerMaxDim || w->cols > kLayerMaxDim)
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: weights of %d x %d", op, w->rows, w->cols);
     if (w->rows > 0 && (!w->d_q || !w->d_scale))
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: a null pointer in the weights", op);

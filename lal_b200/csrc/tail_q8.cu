@@ -530,7 +530,7 @@ int lal_tail_add_rms_norm_q8(const void *d_x, int64_t x_stride, const void *d_re
     static const char *op = "add_rms_norm_q8";
     const int size = dtype_size(dtype);
     if (size == 0) return layer_fail(LAL_TAIL_ERR_ARG, "%s: dtype %d", op, dtype);
-    if (rows < 0 || n_embd < 1)
+    if (rows < 0 || n_embd < 1 || n_embd > kLayerMaxDim)
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: %d rows of %d", op, rows, n_embd);
     if (!(eps >= 0.0f && eps <= kFltMax))
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: eps %g", op, (double)eps);
@@ -572,7 +572,7 @@ int lal_tail_swiglu_q8(const void *d_gate, int64_t gate_stride, const void *d_up
     static const char *op = "swiglu_q8";
     const int size = dtype_size(dtype);
     if (size == 0) return layer_fail(LAL_TAIL_ERR_ARG, "%s: dtype %d", op, dtype);
-    if (rows < 0 || n < 1) return layer_fail(LAL_TAIL_ERR_ARG, "%s: %d rows of %d", op, rows, n);
+    if (rows < 0 || n < 1 || n > kLayerMaxDim) return layer_fail(LAL_TAIL_ERR_ARG, "%s: %d rows of %d", op, rows, n);
     if (rows == 0) return LAL_TAIL_OK;
     if (!d_gate || !d_up || !d_q || !d_scale)
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: a null pointer", op);

@@ -632,3 +632,58 @@ def test_another_stream_and_thread():
     for b, w in zip(blocks, want):
         for got, one in zip(b.outputs(), w):
             assert torch.equal(got, one)
+
+
+FIRST_CALLS_IN_A_CAPTURE = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+from test_gpu_layer_ops import Block
+
+b = Block(%d, 1024, 1536, 64, "bf16")  # (its weights are quantized before)
+b.feed(3)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    b.run(torch.cuda.current_stream().cuda_stream)
+g.replay()
+torch.cuda.synchronize()
+b.check()
+print("captured")
+"""
+
+
+@pytest.mark.parametrize("streams", [1, 12, 40])
+def test_first_calls_of_a_process_in_a_capture(streams):
+    import os
+    import subprocess
+    import sys
+
+    tests = os.path.dirname(os.path.abspath(__file__))
+    code = FIRST_CALLS_IN_A_CAPTURE % (os.path.dirname(tests), tests, streams)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_results_do_not_depend_on_other_streams_values():
+    """A stream's results are the same bits whatever the other vectors hold,
+    and in every run."""
+    rng = np.random.default_rng(12)
+    for streams in (2, 9, 20, 64, 70):
+        q, scale, low = random_weights(rng, 300, 1000, 64, True)
+        d = Weights(300, 1000, 64, True, q, scale, low)
+        xq, sx = vectors(rng, streams, 1000)
+        first = run_matvec(xq, sx, d, "f32")
+        assert torch.equal(first, run_matvec(xq, sx, d, "f32"))
+        other, so = vectors(rng, streams, 1000)
+        other[1], so[1] = xq[1], sx[1]
+        assert torch.equal(first[1], run_matvec(other, so, d, "f32")[1])
+
+
+@pytest.mark.parametrize("streams,rows,cols", [(24, 40000, 1000), (32, 19001, 2100), (17, 152064, 260), (30, 12000, 3585),
+                                               (16, 120000, 300), (8, 152064, 288), (48, 20000, 1500)])
+def test_matvec_many_rows(streams, rows, cols):
+    """More rows than a wave of tiles, ranges and tiles that end unevenly."""
+    rng = np.random.default_rng(rows)
+    check_matvec(rng, streams, rows, cols, 32, True, "bf16", 0)
+    check_matvec(rng, streams, rows, cols, 128, False, "f32", 3)

@@ -22,7 +22,7 @@ def norm(**k):
 
 
 @pytest.mark.parametrize("k", [
-    dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(n_embd=0), dict(n_embd=-5),
+    dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(n_embd=0), dict(n_embd=-5), dict(n_embd=2 ** 30 + 1),
     dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")),
     dict(d_x=None), dict(d_norm_w=None), dict(d_q=None), dict(d_scale=None),
     dict(d_residual=F),                        # a residual needs d_h
@@ -46,7 +46,7 @@ def swiglu(**k):
 
 
 @pytest.mark.parametrize("k", [
-    dict(dtype=7), dict(rows=-1), dict(n=0), dict(d_gate=None), dict(d_up=None), dict(d_q=None),
+    dict(dtype=7), dict(rows=-1), dict(n=0), dict(n=2 ** 31 - 1), dict(d_gate=None), dict(d_up=None), dict(d_q=None),
     dict(d_scale=None), dict(gate_stride=63), dict(up_stride=1), dict(q_stride=0), dict(d_gate=A + 1),
     dict(d_up=B + 1, dtype=L.LAL_TAIL_F16), dict(d_scale=E + 1), dict(d_q=A), dict(d_scale=B), dict(d_q=E - 1),
 ])
@@ -61,7 +61,7 @@ def weights(d_q=A, d_scale=B, d_min=None, rows=4, cols=64, group=32):
 
 
 BAD_WEIGHTS = [dict(d_q=None), dict(d_scale=None), dict(d_q=A + 8), dict(d_scale=B + 1), dict(d_min=D + 1),
-               dict(rows=-1), dict(cols=0), dict(cols=-32), dict(group=0), dict(group=16), dict(group=256)]
+               dict(rows=-1), dict(cols=0), dict(cols=-32), dict(rows=2 ** 31 - 1), dict(cols=2 ** 31 - 1), dict(group=0), dict(group=16), dict(group=256)]
 
 
 @pytest.mark.parametrize("k", BAD_WEIGHTS)
