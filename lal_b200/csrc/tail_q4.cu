@@ -119,6 +119,7 @@ inline long long q4_ctas(int rows, int cols) { return ((long long)rows * q4_row_
 
 template <typename T, int kGroup, bool kMin>
 __global__ void __launch_bounds__(32 * kQ4Warps) quantize_q4_kernel(const ConvertParams p) {
+    after_previous();
     const int lane = threadIdx.x & 31, nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
     constexpr bool kRow8 = sizeof(T) == 2;
     const int per_row = q4_row_warps(p.cols);
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps) quantize_q4_kernel(const Conver
 
 template <typename T, int kGroup, bool kMin>
 __global__ void __launch_bounds__(32 * kQ4Warps) dequantize_q4_kernel(const ConvertParams p) {
+    after_previous();
     const int lane = threadIdx.x & 31, nb = q4_blocks(p.cols), groups = (p.cols + kGroup - 1) / kGroup;
     const int per_row = q4_row_warps(p.cols);
     const long long at = (long long)blockIdx.x * kQ4Warps + (threadIdx.x >> 5);
@@ -520,6 +522,11 @@ __global__ void __launch_bounds__(32 * mma_warps(kMany), mma_ctas(kMT, kNT)) q4_
                 }
             }
         };
+        /* weights on their way into L2 while the kernel before ends; nothing is read yet */
+#pragma unroll
+        for (int j = 0; j < 4 * kMT; ++j)
+            if (wk * kStageBlocks + w_k < nb && w_r + 4 * j < rows) prefetch_l2(w_src + j * w_step);
+        after_previous();
         int ahead = wk;
 #pragma unroll
         for (int i = 0; i < kDepth - 1; ++i, ahead += warps_k) {
@@ -601,6 +608,8 @@ __global__ void __launch_bounds__(32 * mma_warps(kMany), mma_ctas(kMT, kNT)) q4_
             slot = slot + 1 == kDepth ? 0 : slot + 1;
         }
         cp_async_wait<0>();
+    } else {
+        after_previous();
     }
     if (warps_k == 1) {
         if (live) store_tile(p, b0, nx, row0, min(height, p.rows - row0), acc);
@@ -643,9 +652,9 @@ cudaError_t launch_mma(const MatvecParams &p, int x_base, int num_sms, cudaStrea
     constexpr int smem = Stage::kSmem;
     const cudaError_t e = raise_smem((const void *)q4_mma_kernel<kMT, kNT, kGroup, kMin, kMany>, smem);
     if (e != cudaSuccess) return e;
-    q4_mma_kernel<kMT, kNT, kGroup, kMin, kMany>
-        <<<dim3((n + per - 1) / per, (p.streams - x_base + 8 * kNT - 1) / (8 * kNT)), 32 * kWarps, smem, st>>>(p, x_base, wk, height);
-    return cudaGetLastError();
+    return launch_early(q4_mma_kernel<kMT, kNT, kGroup, kMin, kMany>,
+                        dim3((n + per - 1) / per, (p.streams - x_base + 8 * kNT - 1) / (8 * kNT)), 32 * kWarps, smem, st, 1, p,
+                        x_base, wk, height);
 }
 
 /* ---- nine streams and more: tcgen05.mma kind::i8 ----
@@ -822,6 +831,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    after_previous();
     const uint32_t tmem = sh.tmem, tmem_d = tmem + 64 * kTcA; /* the A operands, then the accumulators */
 
     float acc[kMine]; /* of an epilogue thread */
@@ -1141,18 +1151,9 @@ cudaError_t launch_tc(const MatvecParams &p, int x_base, int chunks, int num_sms
     constexpr int smem = tc_smem<kN, kGroup, kMin>();
     cudaError_t e = raise_smem(fn, smem);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(splits > 1 ? tiles * splits : std::min(tiles, num_sms)), (unsigned)chunks);
-    cfg.blockDim = dim3(32 * kTcWarps);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)splits;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, q4_tc_kernel<kN, kGroup, kMin>, p, splits, x_base);
+    return launch_early(q4_tc_kernel<kN, kGroup, kMin>,
+                        dim3((unsigned)(splits > 1 ? tiles * splits : std::min(tiles, num_sms)), (unsigned)chunks), 32 * kTcWarps,
+                        smem, st, splits, p, splits, x_base);
 }
 
 /* ---- many streams: the same products, the vectors shared by a CTA ----
@@ -1263,6 +1264,7 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
         }
         cp_async_commit();
     };
+    after_previous();
     for (int i = 0; i < kWideDepth - 1; ++i) load();
 
     /* ---- products ---- */
@@ -1390,8 +1392,8 @@ cudaError_t launch_wide(const MatvecParams &p, int x_base, int num_sms, cudaStre
     h.height = (h.range + n * Stage::kWarps - 1) / (n * Stage::kWarps);
     const cudaError_t e = raise_smem((const void *)q4_wide_kernel<kGroup, kMin>, Stage::kSmem);
     if (e != cudaSuccess) return e;
-    q4_wide_kernel<kGroup, kMin><<<(p.rows + h.range - 1) / h.range, Stage::kThreads, Stage::kSmem, st>>>(p, h, x_base);
-    return cudaGetLastError();
+    return launch_early(q4_wide_kernel<kGroup, kMin>, dim3((p.rows + h.range - 1) / h.range), Stage::kThreads, Stage::kSmem, st,
+                        1, p, h, x_base);
 }
 
 /* Which kernel.  Measured on a B200, us:
@@ -1437,12 +1439,9 @@ template <int kGroup> cudaError_t launch_matvec(const MatvecParams &p, int num_s
 /* one of the conversions' kernels by type, group and minimum */
 template <typename T, int kGroup>
 cudaError_t launch_convert(const ConvertParams &p, bool back, cudaStream_t st) {
-    const unsigned n = (unsigned)q4_ctas(p.rows, p.cols);
-    if (back && p.min) dequantize_q4_kernel<T, kGroup, true><<<n, 32 * kQ4Warps, 0, st>>>(p);
-    else if (back) dequantize_q4_kernel<T, kGroup, false><<<n, 32 * kQ4Warps, 0, st>>>(p);
-    else if (p.min) quantize_q4_kernel<T, kGroup, true><<<n, 32 * kQ4Warps, 0, st>>>(p);
-    else quantize_q4_kernel<T, kGroup, false><<<n, 32 * kQ4Warps, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_early(back ? (p.min ? dequantize_q4_kernel<T, kGroup, true> : dequantize_q4_kernel<T, kGroup, false>)
+                             : (p.min ? quantize_q4_kernel<T, kGroup, true> : quantize_q4_kernel<T, kGroup, false>),
+                        dim3((unsigned)q4_ctas(p.rows, p.cols)), 32 * kQ4Warps, 0, st, 1, p);
 }
 template <typename T> cudaError_t launch_convert(const ConvertParams &p, bool back, cudaStream_t st) {
     return p.group == 32   ? launch_convert<T, 32>(p, back, st)

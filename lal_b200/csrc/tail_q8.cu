@@ -400,6 +400,7 @@ template <typename Row> struct RowQuant {
  * registers between the statistics and the quantizer. */
 template <typename Row, int kC, int kMaxThreads, int kMinCtas, bool kCluster>
 __global__ void __launch_bounds__(kMaxThreads, kMinCtas) row_q8_kernel(const RowParams p) {
+    after_previous();
     __shared__ RowShared sh;
     const int parts = kCluster ? p.parts : 1, part = kCluster ? blockIdx.x % parts : 0;
     const int at = kCluster ? blockIdx.x / parts : blockIdx.x;
@@ -443,6 +444,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) row_q8_kernel(const Row
 /* Rows longer than that: one CTA, and every element is visited again. */
 constexpr int kLongThreads = 512;
 template <typename Row> __global__ void __launch_bounds__(kLongThreads) row_q8_long_kernel(const RowParams p) {
+    after_previous();
     __shared__ RowShared sh;
     const Row row(p, blockIdx.x);
     double sum = 0.0;
@@ -475,21 +477,9 @@ cudaError_t launch_parts(RowParams p, int rows, int parts, cudaStream_t st) {
     const int eights = (p.n + 7) / 8;
     const int threads = ((eights + parts * kC - 1) / (parts * kC) + 31) / 32 * 32;
     p.parts = parts;
-    if (parts == 1) {
-        row_q8_kernel<Row, kC, kMaxThreads, kMinCtas, false><<<rows, threads, 0, st>>>(p);
-        return cudaGetLastError();
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * parts));
-    cfg.blockDim = dim3(threads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)parts;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, row_q8_kernel<Row, kC, kMaxThreads, kMinCtas, true>, p);
+    return launch_early(parts == 1 ? row_q8_kernel<Row, kC, kMaxThreads, kMinCtas, false>
+                                   : row_q8_kernel<Row, kC, kMaxThreads, kMinCtas, true>,
+                        dim3((unsigned)(rows * parts)), threads, 0, st, parts, p);
 }
 
 constexpr int kFewN = 8192, kFewPart = 2048;
@@ -505,8 +495,7 @@ template <typename Row> cudaError_t launch_row(RowParams p, int rows, int num_sm
         if (Row::kNorm) return launch_parts<Row, 2, 512, 2>(p, rows, (p.n + 8191) / 8192, st);
         if (p.n <= kMaxParts * 4096) return launch_parts<Row, 2, 256, 5>(p, rows, (p.n + 4095) / 4096, st);
     }
-    row_q8_long_kernel<Row><<<rows, kLongThreads, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_early(row_q8_long_kernel<Row>, dim3((unsigned)rows), kLongThreads, 0, st, 1, p);
 }
 
 /* kWide where every row of every buffer begins at a 16-byte boundary (q: 8)
