@@ -352,34 +352,15 @@ __device__ __forceinline__ void mma_s8_zero(int (&c)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
 }
 
-/* n (0 to 16) columns c0 .. of a vector's row to 16 bytes of shared memory,
- * zeros behind them.  Rows that are not aligned to 16 bytes are read as aligned
- * words and shifted, byte by byte at the row's ends (no byte outside the row is
- * read). */
-__device__ __forceinline__ void stage_x16(uint8_t *dst, const int8_t *row, int c0, int cols, bool aligned) {
-    const int n = max(0, min(16, cols - c0));
-    const int8_t *src = row + (n > 0 ? c0 : 0);
-    if (aligned) {
-        cp_async16_l1(smem_u32(dst), src, n);
-        return;
-    }
-    uint32_t v[4] = {0, 0, 0, 0};
-    if (c0 >= 4 && c0 + 20 <= cols) {
-        const unsigned off = (unsigned)((uintptr_t)src & 3);
-        const uint32_t *w = (const uint32_t *)(src - off);
-        uint32_t a = __ldg(w);
+/* 16 columns c0 .. of kCount vectors, `step` bytes apart and aligned to 16 bytes,
+ * of which n exist (of vector j to dst(j)); zeros behind their end. */
+template <int kCount, typename Dst>
+__device__ __forceinline__ void stage_x(Dst dst, const int8_t *x, size_t step, int n, int c0, int cols) {
+    const int bytes = max(0, min(16, cols - c0));
+    if (bytes > 0) x += c0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t b = __ldg(w + i + 1);
-            v[i] = __funnelshift_r(a, b, 8 * off);
-            a = b;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < n) v[i / 4] |= (uint32_t)(uint8_t)__ldg(src + i) << (8 * (i % 4));
-    }
-    *(uint4 *)dst = make_uint4(v[0], v[1], v[2], v[3]);
+    for (int j = 0; j < kCount; ++j, x += step)
+        if (j < n) cp_async16_l1(smem_u32(dst(j)), x, bytes);
 }
 
 __device__ __forceinline__ void store_y(const MatvecParams &p, int b, int row, float v) {
@@ -430,30 +411,34 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
                  : "memory");
 }
 
-/* Stages of a warp's ring, warps of a CTA, CTAs of an SM.  kMany (32 rows by 16
- * streams, tiles for several waves): more warps with shorter rings; 62 us
- * against 74 for 152064x3584 and sixteen streams, but 30 against 17 for
- * 37888x3584, one wave. */
-constexpr int mma_depth(bool many) { return many ? 2 : 3; }
-constexpr int mma_warps(bool many) { return many ? 12 : 8; }
-constexpr int mma_ctas(int mt, int nt) { return mt * nt == 1 ? 2 : 1; }
+/* How a warp's ring is filled.  kAligned: vectors and rows of scales begin at
+ * 16-byte boundaries (scales: of a stage's size) and lie as ldmatrix wants
+ * them.  kAny: the aligned 16-byte pieces around them are copied as they are,
+ * and their offsets are taken at the reading, so these copies are asynchronous
+ * too.  kMany (aligned, 32 rows a warp, tiles for several waves): more warps
+ * with shorter rings; 62 us against 74 for 152064x3584 and sixteen streams,
+ * but 30 against 17 for 37888x3584, one wave. */
+enum MmaFill { kAligned, kMany, kAny };
 
 /* What a warp's ring holds a stage: weights of 16 kMT rows, their scales (and
  * minima), the part of 8 kNT vectors. */
-template <int kMT, int kNT, int kGroup, bool kMin, bool kMany> struct MmaStage {
+template <int kMT, int kNT, int kGroup, bool kMin, MmaFill kFill> struct MmaStage {
     static constexpr int kGroups = kStageBlocks * kQ4Block / kGroup;
-    static constexpr int kScale = 16 * kMT * kGroups * 2;
+    static constexpr int kSRow = kFill == kAny ? 32 : kGroups * 2;                   /* bytes of a row's scales */
+    static constexpr int kXRow = kStageBlocks * 32 + (kFill == kAny ? 32 : 0);      /* of a vector's part */
+    static constexpr int kScale = 16 * kMT * kSRow;
     static constexpr int kS = 16 * kMT * 128, kX = (kS + (kMin ? 2 : 1) * kScale + 127) / 128 * 128;
-    static constexpr int kBytes = (kX + 8 * kNT * kStageBlocks * 32 + 127) / 128 * 128;
-    static constexpr int kDepth = mma_depth(kMany), kWarps = mma_warps(kMany), kCtas = mma_ctas(kMT, kNT);
+    static constexpr int kBytes = (kX + 8 * kNT * kXRow + 127) / 128 * 128;
+    static constexpr int kWarps = kFill == kMany ? 12 : 8, kCtas = kMT * kNT == 1 ? 2 : 1;
+    static constexpr int kDepth = kFill == kMany || (kFill == kAny && kMT * kNT != 2) ? 2 : 3;
     static constexpr int kSmem = kWarps * kDepth * kBytes;
     static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "CTAs of an SM");
 };
 
-template <int kMT, int kNT, int kGroup, bool kMin, bool kMany>
-__global__ void __launch_bounds__(32 * mma_warps(kMany), mma_ctas(kMT, kNT)) q4_mma_kernel(const MatvecParams p, int x_base, int warps_k, int height) {
+template <int kMT, int kNT, int kGroup, bool kMin, MmaFill kFill>
+__global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2 : 1) q4_mma_kernel(const MatvecParams p, int x_base, int warps_k, int height) {
     extern __shared__ __align__(128) uint8_t smem[];
-    using Stage = MmaStage<kMT, kNT, kGroup, kMin, kMany>;
+    using Stage = MmaStage<kMT, kNT, kGroup, kMin, kFill>;
     constexpr int kDepth = Stage::kDepth, kWarps = Stage::kWarps;
     constexpr int kPer = kGroup / kQ4Block, kGroups = Stage::kGroups; /* blocks of a group, groups of a stage */
     constexpr int kRows = 16 * kMT, kStreams = 8 * kNT;
@@ -480,11 +465,8 @@ __global__ void __launch_bounds__(32 * mma_warps(kMany), mma_ctas(kMT, kNT)) q4_
         const int x_n = lane >> 4, x_c = lane & 15;
         const int8_t *x_src = p.x + (size_t)(b0 + x_n) * p.x_stride;
         const size_t x_step = (size_t)2 * p.x_stride;
-        const bool x_aligned = (((uintptr_t)p.x | (uintptr_t)p.x_stride) & 15) == 0;
-        /* a row's scales of a stage, one copy where all rows' are aligned to it: lane has row lane (+ 16: a minimum's) */
+        /* a row's scales of a stage, one copy (kAny: two): lane has rows lane, + 32, the minima after the scales */
         constexpr int kCopies = kRows * (kMin ? 2 : 1);
-        const bool s_aligned =
-            (((uintptr_t)p.scale | (kMin ? (uintptr_t)p.min : 0) | (uintptr_t)(groups * 2)) & (2 * kGroups - 1)) == 0;
         auto load = [&](int st, int slot) {
             const uint32_t base = slot * Stage::kBytes;
             const int k0 = st * kStageBlocks;
@@ -495,30 +477,47 @@ __global__ void __launch_bounds__(32 * mma_warps(kMany), mma_ctas(kMT, kNT)) q4_
             }
             w_src += (size_t)warps_k * (kStageBlocks * 16);
             const int c0 = k0 * kQ4Block + x_c * 16;
-            uint8_t *const x_to = ring + base + Stage::kX + x_n * 256;
-            const int8_t *x = x_src;
-            if (x_aligned && c0 + 16 <= p.cols) {
-#pragma unroll
-                for (int j = 0; j < 4 * kNT; ++j, x += x_step)
-                    if (x_n + 2 * j < nx)
-                        cp_async16_l1(smem_u32(x_to + j * 512 + ((x_c ^ ((x_n + 2 * j) & 7)) << 4)), x + c0, 16);
+            uint8_t *const x_to = ring + base + Stage::kX + x_n * Stage::kXRow;
+            if constexpr (kFill != kAny) {
+                stage_x<4 * kNT>([&](int j) { return x_to + j * 512 + ((x_c ^ ((x_n + 2 * j) & 7)) << 4); }, x_src, x_step,
+                                 (nx - x_n + 1) >> 1, c0, p.cols);
             } else {
-#pragma unroll 1
-                for (int j = 0; x_n + 2 * j < nx; ++j, x += x_step)
-                    stage_x16(x_to + j * 512 + ((x_c ^ ((x_n + 2 * j) & 7)) << 4), x, c0, p.cols, x_aligned);
+                /* pieces x_c, and by the last lane of a row the seventeenth, from the boundary at or before column 256 st */
+                const int8_t *x = x_src;
+#pragma unroll
+                for (int j = 0; j < 4 * kNT; ++j, x += x_step) {
+                    if (x_n + 2 * j >= nx) break;
+                    const int8_t *from = x + k0 * kQ4Block, *end = x + p.cols;
+                    from -= (uintptr_t)from & 15;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int piece = e ? 16 : x_c;
+                        if (e && x_c != 15) break;
+                        const int8_t *src = from + piece * 16;
+                        const int n = (int)max(0LL, min(16LL, (long long)(end - src)));
+                        cp_async16_l1(smem_u32(x_to + j * 2 * Stage::kXRow + piece * 16), n > 0 ? src : from, n);
+                    }
+                }
             }
             const int g0 = st * kGroups;
 #pragma unroll
             for (int i = lane; i < kCopies; i += 32) {
-                const int r = i % kRows;
-                const unsigned short *src =
-                    (const unsigned short *)(i < kRows ? p.scale : p.min) + (size_t)(row0 + min(r, rows - 1)) * groups + g0;
-                unsigned short *to = (unsigned short *)(ring + base + Stage::kS) + i * kGroups;
-                if (s_aligned && g0 + kGroups <= groups) {
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(src), "n"(2 * kGroups) : "memory");
+                const unsigned short *row = (const unsigned short *)(i < kRows ? p.scale : p.min) +
+                                            (size_t)(row0 + min(i % kRows, rows - 1)) * groups;
+                uint8_t *to = ring + base + Stage::kS + i * Stage::kSRow;
+                if constexpr (kFill == kAny) {
+                    const uint8_t *from = (const uint8_t *)(row + g0), *end = (const uint8_t *)(row + groups);
+                    from -= (uintptr_t)from & 15;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int n = (int)max(0LL, min(16LL, (long long)(end - from) - 16 * e));
+                        cp_async16_l1(smem_u32(to + 16 * e), n > 0 ? from + 16 * e : from, n);
+                    }
+                } else if (g0 + kGroups <= groups) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(row + g0), "n"(2 * kGroups) : "memory");
                 } else {
 #pragma unroll
-                    for (int k = 0; k < kGroups; ++k) to[k] = g0 + k < groups ? __ldg(src + k) : 0;
+                    for (int k = 0; k < kGroups; ++k) ((unsigned short *)to)[k] = g0 + k < groups ? __ldg(row + g0 + k) : 0;
                 }
             }
         };
@@ -536,6 +535,17 @@ __global__ void __launch_bounds__(32 * mma_warps(kMany), mma_ctas(kMT, kNT)) q4_
         /* ldmatrix addresses: rows lane mod 16, block lane / 16 of a pair; vectors lane mod 8, piece lane / 8 of a pair's four */
         const uint32_t a_at = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
         const uint32_t x_at = Stage::kX + (lane & 7) * 256 + (((lane >> 3) ^ (lane & 7)) << 4);
+        /* kAny: this lane's first word of vector 8 n + g, and the bits to shift it by */
+        uint32_t x_any[kNT], x_shift[kNT];
+        if constexpr (kFill == kAny) {
+#pragma unroll
+            for (int n = 0; n < kNT; ++n) {
+                const int v = min(8 * n + g, nx - 1); /* vectors that are not there: any, their sums are dropped */
+                const uint32_t off = (uint32_t)(uintptr_t)(p.x + (size_t)(b0 + v) * p.x_stride) & 15;
+                x_any[n] = Stage::kX + v * Stage::kXRow + (off & ~3u) + 4 * t;
+                x_shift[n] = 8 * (off & 3);
+            }
+        }
         int slot = 0;
         for (int st = wk; st < stages; st += warps_k, ahead += warps_k) {
             cp_async_wait<kDepth - 2>();
@@ -549,13 +559,25 @@ __global__ void __launch_bounds__(32 * mma_warps(kMany), mma_ctas(kMT, kNT)) q4_
                 __half one[kGroups];
                 __device__ Row() {}
             } scale[kMT][2], low[kMT][2]; /* of rows g and g + 8 */
-            const Pack *sc = (const Pack *)(ring + slot * Stage::kBytes + Stage::kS) + g;
+            const uint8_t *sc = ring + slot * Stage::kBytes + Stage::kS + g * Stage::kSRow;
 #pragma unroll
             for (int m = 0; m < kMT; ++m)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    scale[m][h].all = sc[16 * m + 8 * h];
-                    if (kMin) low[m][h].all = sc[kRows + 16 * m + 8 * h];
+                    const uint8_t *at_s = sc + (16 * m + 8 * h) * Stage::kSRow;
+                    if constexpr (kFill != kAny) {
+                        scale[m][h].all = *(const Pack *)at_s;
+                        if (kMin) low[m][h].all = *(const Pack *)(at_s + Stage::kScale);
+                    } else {
+                        /* rows that are not there: any offset within the copy */
+                        const size_t i = (size_t)(row0 + min(g + 16 * m + 8 * h, rows - 1)) * groups + st * kGroups;
+                        const uint32_t off = (uint32_t)(uintptr_t)(p.scale + i) & 15, off_m = (uint32_t)(uintptr_t)(p.min + i) & 15;
+#pragma unroll
+                        for (int k = 0; k < kGroups; ++k) {
+                            scale[m][h].one[k] = *(const __half *)(at_s + off + 2 * k);
+                            if (kMin) low[m][h].one[k] = *(const __half *)(at_s + Stage::kScale + off_m + 2 * k);
+                        }
+                    }
                 }
             int c[kMT][kNT][4], cx[kNT][4];
 #pragma unroll
@@ -565,7 +587,16 @@ __global__ void __launch_bounds__(32 * mma_warps(kMany), mma_ctas(kMT, kNT)) q4_
 #pragma unroll
                 for (int m = 0; m < kMT; ++m) ldmatrix4(w[m], (at + a_at + m * 2048) ^ (pair << 5));
 #pragma unroll
-                for (int n = 0; n < kNT; ++n) ldmatrix4(x[n], ((at + x_at + n * 2048) ^ ((pair & 1) << 6)) + (pair >> 1) * 128);
+                for (int n = 0; n < kNT; ++n) {
+                    if constexpr (kFill != kAny) {
+                        ldmatrix4(x[n], ((at + x_at + n * 2048) ^ ((pair & 1) << 6)) + (pair >> 1) * 128);
+                    } else {
+                        const uint8_t *from = ring + slot * Stage::kBytes + x_any[n] + pair * 64;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            x[n][i] = __funnelshift_r(*(const uint32_t *)(from + 16 * i), *(const uint32_t *)(from + 16 * i + 4), x_shift[n]);
+                    }
+                }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const int block = 2 * pair + k;
@@ -637,22 +668,22 @@ __global__ void __launch_bounds__(32 * mma_warps(kMany), mma_ctas(kMT, kNT)) q4_
     }
 }
 
-template <int kMT, int kNT, int kGroup, bool kMin, bool kMany>
+template <int kMT, int kNT, int kGroup, bool kMin, MmaFill kFill>
 cudaError_t launch_mma(const MatvecParams &p, int x_base, int num_sms, cudaStream_t st) {
-    /* warps of a row tile: enough that the tiles' warps fill the SMs, no more than there are stages */
-    using Stage = MmaStage<kMT, kNT, kGroup, kMin, kMany>;
+    /* warps of a row tile: as many as fit the SMs at once, no more than there are stages */
+    using Stage = MmaStage<kMT, kNT, kGroup, kMin, kFill>;
     constexpr int kRows = 16 * kMT, kWarps = Stage::kWarps, kWarpsSm = Stage::kCtas * kWarps;
     const int tiles = (p.rows + kRows - 1) / kRows, stages = (q4_blocks(p.cols) + kStageBlocks - 1) / kStageBlocks;
     int wk = 1;
-    while (!kMany && wk < kWarps && 2 * wk <= stages && (long long)tiles * wk < (long long)kWarpsSm * num_sms) wk *= 2;
+    while (kFill != kMany && wk < kWarps && 2 * wk <= stages && (long long)tiles * 2 * wk <= (long long)kWarpsSm * num_sms) wk *= 2;
     /* rows of a tile: fewer than it holds where that gives every SM some */
     const int at_once = num_sms * (kWarpsSm / wk), waves = (tiles + at_once - 1) / at_once;
     const int height = waves > 1 ? kRows : std::max((p.rows + at_once - 1) / at_once, std::min(p.rows, kRows / 2));
     const int n = (p.rows + height - 1) / height, per = kWarps / wk;
     constexpr int smem = Stage::kSmem;
-    const cudaError_t e = raise_smem((const void *)q4_mma_kernel<kMT, kNT, kGroup, kMin, kMany>, smem);
+    const cudaError_t e = raise_smem((const void *)q4_mma_kernel<kMT, kNT, kGroup, kMin, kFill>, smem);
     if (e != cudaSuccess) return e;
-    return launch_early(q4_mma_kernel<kMT, kNT, kGroup, kMin, kMany>,
+    return launch_early(q4_mma_kernel<kMT, kNT, kGroup, kMin, kFill>,
                         dim3((n + per - 1) / per, (p.streams - x_base + 8 * kNT - 1) / (8 * kNT)), 32 * kWarps, smem, st, 1, p,
                         x_base, wk, height);
 }
@@ -903,21 +934,19 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
         /* ---- accumulators: scaled and added ---- */
         const int quad = warp & 3, part = (warp - kTcUnpack) >> 2;
         const uint32_t lanes = tmem_d + ((uint32_t)(quad * 32) << 16) + part * kMine;
-        /* a row's scales (and minima) of a stage, one load where all rows' are aligned to it */
+        /* a row's scales (and minima) of a stage */
         using Pack = std::conditional_t<kGroups == 8, uint4, std::conditional_t<kGroups == 4, uint2, uint32_t>>;
         union Row {
             Pack all;
             unsigned short one[kGroups];
             __device__ Row() {}
         } scale, low, scale_next, low_next;
-        const bool s_aligned =
-            (((uintptr_t)p.scale | (kMin ? (uintptr_t)p.min : 0) | (uintptr_t)(groups * 2)) & (2 * kGroups - 1)) == 0;
         TcWalk ahead(tile0, st0);
         auto load_scales = [&] {
             if (ahead.n < total) {
                 const int row = min(ahead.tile * 128 + quad * 32 + lane, p.rows - 1), g0 = ahead.st * kGroups;
                 const size_t at = (size_t)row * groups + g0;
-                if (s_aligned && g0 + kGroups <= groups) {
+                if (g0 + kGroups <= groups) {
                     scale_next.all = __ldg((const Pack *)(p.scale + at));
                     if (kMin) low_next.all = __ldg((const Pack *)(p.min + at));
                 } else {
@@ -1040,7 +1069,6 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
     } else {
         /* ---- vectors, and (with minima) their sums ---- */
         const int lw = warp - kTcIssue - 1;
-        const bool x_aligned = (((uintptr_t)p.x | (uintptr_t)p.x_stride) & 15) == 0;
         /* a loader warp has every kTcLoad-th pair of rows: 16 lanes a row */
         const int n0 = lw * 2 + (lane >> 4);
         const int8_t *x0 = p.x + (size_t)(b0 + min(n0, nx - 1)) * p.x_stride;
@@ -1053,13 +1081,10 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                 if (round > 0 && !tc_wait(&sh.x_empty[xs], (round & 1) ^ 1, abort_flag)) return false;
                 const int c0 = ahead.st * kStageBlocks * kQ4Block + (lane & 15) * 16;
                 uint8_t *dst = xring + xs * tc_x_stage(kN) + d0;
-                const int8_t *x = x0;
-                if (x_aligned && c0 + 16 <= p.cols) {
-                    x += c0;
-                    for (int n = n0; n < nx; n += 2 * kTcLoad, x += x_step, dst += 1024) cp_async16_l1(smem_u32(dst), x, 16);
-                } else {
-                    for (int n = n0; n < nx; n += 2 * kTcLoad, x += x_step, dst += 1024) stage_x16(dst, x, c0, p.cols, x_aligned);
-                }
+                const int n = (nx - n0 + 2 * kTcLoad - 1) / (2 * kTcLoad); /* this lane's vectors, four at a time */
+                stage_x<4>([&](int j) { return dst + j * 1024; }, x0, x_step, min(n, 4), c0, p.cols);
+                if (n > 4)
+                    stage_x<4>([&](int j) { return dst + 4096 + j * 1024; }, x0 + 4 * x_step, x_step, n - 4, c0, p.cols);
             }
             ahead.next(st0, st1, tile_step);
             cp_async_commit();
@@ -1207,9 +1232,6 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
     const uint32_t x_to = x_ring + x_n * 256 + ((x_c ^ (x_n & 7)) << 4);
     const int8_t *const x_src = p.x + (size_t)(b0 + min(x_n, nx - 1)) * p.x_stride;
     const size_t x_step = (size_t)kXRows * p.x_stride;
-    const bool x_aligned = (((uintptr_t)p.x | (uintptr_t)p.x_stride) & 15) == 0;
-    const bool s_aligned =
-        (((uintptr_t)p.scale | (kMin ? (uintptr_t)p.min : 0) | (uintptr_t)(groups * 2)) & (2 * kGroups - 1)) == 0;
     size_t s_row = 0;
     int l_row = first + warp * h.height, l_st = 0, l_slot = 0, l_left = total, l_rows = 0;
     auto load = [&] {
@@ -1230,24 +1252,15 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
             w_src += kStageBlocks * 16;
             const int c0 = k0 * kQ4Block + x_c * 16;
             const uint32_t to = x_to + l_slot * Stage::kX;
-            if (x_aligned && c0 + 16 <= p.cols) {
-                const int8_t *x = x_src + c0;
-#pragma unroll
-                for (int j = 0; j < (8 * kNT + kXRows - 1) / kXRows; ++j, x += x_step)
-                    if (x_n + kXRows * j < nx) cp_async16_l1(to + j * (kXRows * 256), x, 16);
-            } else {
-                const int8_t *x = x_src;
-#pragma unroll 1
-                for (int j = 0; x_n + kXRows * j < nx; ++j, x += x_step)
-                    stage_x16(smem + (to - x_ring) + j * (kXRows * 256), x, c0, p.cols, x_aligned);
-            }
+            stage_x<8 * kNT / kXRows>([&](int j) { return smem + (to - x_ring) + j * (kXRows * 256); }, x_src, x_step,
+                                      (nx - x_n + kXRows - 1) / kXRows, c0, p.cols);
             if (lane < l_rows) {
                 const int g0 = l_st * kGroups;
 #pragma unroll
                 for (int m = 0; m < (kMin ? 2 : 1); ++m) {
                     const unsigned short *src = (const unsigned short *)(m ? p.min : p.scale) + s_row + g0;
                     const uint32_t dst = w_ring + base + Stage::kA + m * Stage::kScale + lane * (2 * kGroups);
-                    if (s_aligned && g0 + kGroups <= groups) {
+                    if (g0 + kGroups <= groups) {
                         asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(2 * kGroups) : "memory");
                     } else {
 #pragma unroll
@@ -1407,24 +1420,38 @@ cudaError_t launch_wide(const MatvecParams &p, int x_base, int num_sms, cudaStre
  *   64       3584x18944  g128   45     35.4            29.5
  * so mma up to 16 streams, shared vectors up to 32 where the weights are
  * many, tcgen05 beyond, in chunks of 64 streams and the rest. */
+/* Whether every vector and every row of scales begins where copies of 16 bytes
+ * (scales: of a stage's) may. */
+inline bool all_aligned(const MatvecParams &p) {
+    const int groups = (p.cols + p.group - 1) / p.group, copy = 2 * kStageBlocks * kQ4Block / p.group;
+    return (uintptr_t)p.x % 16 == 0 && (p.streams == 1 || p.x_stride % 16 == 0) &&
+           ((uintptr_t)p.scale | (uintptr_t)p.min | (uintptr_t)groups * 2) % copy == 0;
+}
+
 template <int kGroup, bool kMin>
 cudaError_t launch_streams(const MatvecParams &p, int x_base, int num_sms, cudaStream_t st) {
     const int n = p.streams - x_base;
-    const long long weights = (long long)p.rows * p.cols;
+    const bool large = (long long)p.rows * p.cols >= (long long)num_sms * 256 * 1024;
+    const bool waves = (p.rows + 31) / 32 >= 2 * num_sms * 12; /* of 32 rows, 12 warps an SM */
+    if (!all_aligned(p)) {
+        if (n > 8) return launch_mma<2, 2, kGroup, kMin, kAny>(p, x_base, num_sms, st);
+        return large ? launch_mma<2, 1, kGroup, kMin, kAny>(p, x_base, num_sms, st)
+                     : launch_mma<1, 1, kGroup, kMin, kAny>(p, x_base, num_sms, st);
+    }
     if (n > 32) return launch_tc<kGroup, kMin>(p, x_base, 1, num_sms, st);
-    if (n > 16 && weights >= (long long)num_sms * 256 * 1024) return launch_wide<kGroup, kMin>(p, x_base, num_sms, st);
+    if (n > 16 && large) return launch_wide<kGroup, kMin>(p, x_base, num_sms, st);
     if (n > 8)
-        return (p.rows + 31) / 32 >= 2 * num_sms * mma_warps(true) ? launch_mma<2, 2, kGroup, kMin, true>(p, x_base, num_sms, st)
-                                                                   : launch_mma<2, 2, kGroup, kMin, false>(p, x_base, num_sms, st);
+        return waves ? launch_mma<2, 2, kGroup, kMin, kMany>(p, x_base, num_sms, st)
+                     : launch_mma<2, 2, kGroup, kMin, kAligned>(p, x_base, num_sms, st);
     /* 32 rows a warp share its part of the vectors: fewer instructions, but half the warps.  Eight
-     * streams, groups of 32: 16.3 us against 20.0 for 37888x3584, 6.2 against 5.8 for 5000x1000; groups
-     * of 128, where the instructions do not bound: 61 against 57 for 152064x3584. */
-    if (kGroup == 32 && weights >= (long long)num_sms * 256 * 1024) return launch_mma<2, 1, kGroup, kMin, false>(p, x_base, num_sms, st);
-    return launch_mma<1, 1, kGroup, kMin, false>(p, x_base, num_sms, st);
+     * streams: 16.3 us against 20.0 for 37888x3584, 6.2 against 5.8 for 5000x1000. */
+    if (waves) return launch_mma<2, 1, kGroup, kMin, kMany>(p, x_base, num_sms, st);
+    if (large) return launch_mma<2, 1, kGroup, kMin, kAligned>(p, x_base, num_sms, st);
+    return launch_mma<1, 1, kGroup, kMin, kAligned>(p, x_base, num_sms, st);
 }
 
 template <int kGroup, bool kMin> cudaError_t launch_matvec(const MatvecParams &p, int num_sms, cudaStream_t st) {
-    const int whole = p.streams / kTcStreams;
+    const int whole = all_aligned(p) ? p.streams / kTcStreams : 0;
     if (whole > 0) {
         const cudaError_t e = launch_tc<kGroup, kMin>(p, 0, whole, num_sms, st);
         if (e != cudaSuccess || whole * kTcStreams == p.streams) return e;
