@@ -404,6 +404,18 @@ __device__ __forceinline__ void store_tile(const MatvecParams &p, int b0, int nx
     else store_tile_as<__half>(p, b0, nx, row0, rows, acc);
 }
 
+/* kCount words from an even offset on */
+template <int kCount> __device__ __forceinline__ void shifted_words(uint32_t (&w)[kCount], const uint8_t *from, uint32_t off) {
+    const uint32_t *at = (const uint32_t *)(from + (off & ~3u));
+    uint32_t a = at[0];
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+        const uint32_t b = at[i + 1];
+        w[i] = __funnelshift_r(a, b, 8 * (off & 2));
+        a = b;
+    }
+}
+
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -424,8 +436,9 @@ enum MmaFill { kAligned, kMany, kAny };
  * minima), the part of 8 kNT vectors. */
 template <int kMT, int kNT, int kGroup, bool kMin, MmaFill kFill> struct MmaStage {
     static constexpr int kGroups = kStageBlocks * kQ4Block / kGroup;
-    static constexpr int kSRow = kFill == kAny ? 32 : kGroups * 2;                   /* bytes of a row's scales */
-    static constexpr int kXRow = kStageBlocks * 32 + (kFill == kAny ? 32 : 0);      /* of a vector's part */
+    /* bytes of a row's scales, of a vector's part; kAny: two and seventeen pieces, eight rows in different banks */
+    static constexpr int kSRow = kFill == kAny ? 48 : kGroups * 2;
+    static constexpr int kXRow = kStageBlocks * 32 + (kFill == kAny ? 16 : 0);
     static constexpr int kScale = 16 * kMT * kSRow;
     static constexpr int kS = 16 * kMT * 128, kX = (kS + (kMin ? 2 : 1) * kScale + 127) / 128 * 128;
     static constexpr int kBytes = (kX + 8 * kNT * kXRow + 127) / 128 * 128;
@@ -507,9 +520,11 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
                 uint8_t *to = ring + base + Stage::kS + i * Stage::kSRow;
                 if constexpr (kFill == kAny) {
                     const uint8_t *from = (const uint8_t *)(row + g0), *end = (const uint8_t *)(row + groups);
-                    from -= (uintptr_t)from & 15;
+                    const int off = (int)((uintptr_t)from & 15);
+                    from -= off;
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
+                        if (e && off + 2 * kGroups <= 16) break; /* within the first */
                         const int n = (int)max(0LL, min(16LL, (long long)(end - from) - 16 * e));
                         cp_async16_l1(smem_u32(to + 16 * e), n > 0 ? from + 16 * e : from, n);
                     }
@@ -556,6 +571,7 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
             using Pack = std::conditional_t<kGroups == 8, uint4, std::conditional_t<kGroups == 4, uint2, uint32_t>>;
             union Row {
                 Pack all;
+                uint32_t word[kGroups / 2];
                 __half one[kGroups];
                 __device__ Row() {}
             } scale[kMT][2], low[kMT][2]; /* of rows g and g + 8 */
@@ -572,11 +588,8 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
                         /* rows that are not there: any offset within the copy */
                         const size_t i = (size_t)(row0 + min(g + 16 * m + 8 * h, rows - 1)) * groups + st * kGroups;
                         const uint32_t off = (uint32_t)(uintptr_t)(p.scale + i) & 15, off_m = (uint32_t)(uintptr_t)(p.min + i) & 15;
-#pragma unroll
-                        for (int k = 0; k < kGroups; ++k) {
-                            scale[m][h].one[k] = *(const __half *)(at_s + off + 2 * k);
-                            if (kMin) low[m][h].one[k] = *(const __half *)(at_s + Stage::kScale + off_m + 2 * k);
-                        }
+                        shifted_words(scale[m][h].word, at_s, off);
+                        if (kMin) shifted_words(low[m][h].word, at_s + Stage::kScale, off_m);
                     }
                 }
             int c[kMT][kNT][4], cx[kNT][4];
