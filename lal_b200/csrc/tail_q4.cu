@@ -428,7 +428,7 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
  * them.  kAny: the aligned 16-byte pieces around them are copied as they are,
  * and their offsets are taken at the reading, so these copies are asynchronous
  * too.  kMany (aligned, 32 rows a warp, tiles for several waves): more warps
- * with shorter rings; 62 us against 74 for 152064x3584 and sixteen streams,
+ * with shorter rings; 58 us against 68 for 152064x3584 g128 and sixteen streams,
  * but 30 against 17 for 37888x3584, one wave. */
 enum MmaFill { kAligned, kMany, kAny };
 
@@ -1422,17 +1422,6 @@ cudaError_t launch_wide(const MatvecParams &p, int x_base, int num_sms, cudaStre
                         1, p, h, x_base);
 }
 
-/* Which kernel.  Measured on a B200, us:
- *   streams  weights            mma    shared vectors  tcgen05
- *   8        152064x3584 g128   56     58              123
- *   16       37888x3584  g32    24.1   22.1            55
- *   32       37888x3584  g128   31.4   22.8            33.7
- *   32       3584x18944  g32    33.0   23.6            45.7
- *   32       3584x3584   g32    11.5   14.4            15.4
- *   64       37888x3584  g128   61     43.4            36.2
- *   64       3584x18944  g128   45     35.4            29.5
- * so mma up to 16 streams, shared vectors up to 32 where the weights are
- * many, tcgen05 beyond, in chunks of 64 streams and the rest. */
 /* Whether every vector and every row of scales begins where copies of 16 bytes
  * (scales: of a stage's) may. */
 inline bool all_aligned(const MatvecParams &p) {
@@ -1441,6 +1430,20 @@ inline bool all_aligned(const MatvecParams &p) {
            ((uintptr_t)p.scale | (uintptr_t)p.min | (uintptr_t)groups * 2) % copy == 0;
 }
 
+/* Which kernel for the last (at most 64) streams, from x_base on.  Measured on a
+ * B200, back to back, us:
+ *   streams  weights            mma    shared vectors  tcgen05
+ *   16       152064x3584 g128   58     97              135
+ *   16       37888x3584  g32    25.2   29.2            69.5
+ *   32       37888x3584  g128   29.0   22.3            34.1
+ *   32       37888x3584  g32    46.0   29.8            69.6
+ *   32       3584x3584   g32    10.5   26.8            16.1
+ *   64       37888x3584  g128   56.7                   34.9
+ *   64       37888x3584  g32    85.8                   70.5
+ *   64       3584x3584   g32    19.5                   16.6
+ * so mma up to 16 streams, shared vectors up to 32 where every SM has 128
+ * rows, tcgen05 beyond (and for whole 64s).  What is not aligned takes mma, 16
+ * streams at a time. */
 template <int kGroup, bool kMin>
 cudaError_t launch_streams(const MatvecParams &p, int x_base, int num_sms, cudaStream_t st) {
     const int n = p.streams - x_base;
@@ -1452,12 +1455,13 @@ cudaError_t launch_streams(const MatvecParams &p, int x_base, int num_sms, cudaS
                      : launch_mma<1, 1, kGroup, kMin, kAny>(p, x_base, num_sms, st);
     }
     if (n > 32) return launch_tc<kGroup, kMin>(p, x_base, 1, num_sms, st);
-    if (n > 16 && large) return launch_wide<kGroup, kMin>(p, x_base, num_sms, st);
+    if (n > 16 && p.rows >= 128 * num_sms) return launch_wide<kGroup, kMin>(p, x_base, num_sms, st);
     if (n > 8)
         return waves ? launch_mma<2, 2, kGroup, kMin, kMany>(p, x_base, num_sms, st)
                      : launch_mma<2, 2, kGroup, kMin, kAligned>(p, x_base, num_sms, st);
     /* 32 rows a warp share its part of the vectors: fewer instructions, but half the warps.  Eight
-     * streams: 16.3 us against 20.0 for 37888x3584, 6.2 against 5.8 for 5000x1000. */
+     * streams, us: 13.9 against 18.4 for 37888x3584 g32, 13.0 against 17.1 for 3584x18944 with minima,
+     * 3.4 against 2.9 for 5000x1024 */
     if (waves) return launch_mma<2, 1, kGroup, kMin, kMany>(p, x_base, num_sms, st);
     if (large) return launch_mma<2, 1, kGroup, kMin, kAligned>(p, x_base, num_sms, st);
     return launch_mma<1, 1, kGroup, kMin, kAligned>(p, x_base, num_sms, st);
