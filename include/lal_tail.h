@@ -443,7 +443,8 @@ int lal_tail_dequantize_q4(const lal_tail_q4 *w, void *d_w, int64_t w_stride, in
 /* y[b, r] = d_scale_x[b] * sum over columns c of xq[b, c] * weight[r, c], for
  * n_streams (at most LAL_TAIL_Q4_MAX_STREAMS) 8-bit vectors; y is [n_streams,
  * w->rows] of `dtype`.  The dots of 32 columns are exact integers, their
- * scaled sum is held in fp32.  xq may hold -128.  (Beside
+ * scaled sum is held in fp32.  xq may hold -128.  Vectors and rows of scales at
+ * 16-byte boundaries are read fastest.  (Beside
  * lal_lm_head_int8_range, runtime/lal_q8_kernel.h:463; the 4-bit products of
  * the server's layers.) */
 int lal_tail_q4_matvec(const lal_tail_q4 *w, const int8_t *d_xq, int64_t xq_stride,
