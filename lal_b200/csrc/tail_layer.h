@@ -114,7 +114,9 @@ inline int launched(const char *op, cudaError_t e) {
 #if defined(__CUDACC__)
 /* Launches `kernel` (over clusters of `cluster` CTAs) so that it may begin
  * while the kernel before it on the stream ends: every thread of it calls
- * after_previous() before it reads or writes anything that a call may share. */
+ * after_previous() before it reads or writes anything that a call may share,
+ * and what that kernel may have written is read by ordinary loads: it is not
+ * constant over this kernel's life, as __ldg wants it. */
 template <typename... P, typename... A>
 cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster, A &&...args) {
     cudaLaunchConfig_t cfg = {};

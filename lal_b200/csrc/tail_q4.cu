@@ -59,10 +59,10 @@ __device__ __forceinline__ __half f16_floor(float x) {
 template <typename T> __device__ __forceinline__ void get4(const T *p, int n, bool aligned, float (&v)[4]) {
     if (n >= 4 && aligned) {
         if constexpr (sizeof(T) == 4) {
-            const float4 f = __ldg((const float4 *)p);
+            const float4 f = *(const float4 *)p;
             v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
         } else {
-            const uint2 w = __ldg((const uint2 *)p);
+            const uint2 w = *(const uint2 *)p;
             unpack16<T>(w.x, v[0], v[1]);
             unpack16<T>(w.y, v[2], v[3]);
         }
@@ -71,8 +71,9 @@ template <typename T> __device__ __forceinline__ void get4(const T *p, int n, bo
         for (int i = 0; i < 4; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
     }
 }
-template <typename T> __device__ __forceinline__ void put4(T *p, int n, bool aligned, const float (&v)[4]) {
-    if (n >= 4 && aligned) {
+/* to p, aligned to four elements */
+template <typename T> __device__ __forceinline__ void put4(T *p, int n, const float (&v)[4]) {
+    if (n >= 4) {
         if constexpr (sizeof(T) == 4) {
             *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
         } else {
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps) quantize_q4_kernel(const Conver
         float lo[4], hi[4];
         if constexpr (kRow8) {
             if (p.aligned && c + 8 <= p.cols) {
-                const uint4 x = __ldg((const uint4 *)w);
+                const uint4 x = *(const uint4 *)w;
                 unpack16<T>(x.x, lo[0], lo[1]);
                 unpack16<T>(x.y, lo[2], lo[3]);
                 unpack16<T>(x.z, hi[0], hi[1]);
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps) dequantize_q4_kernel(const Conv
         const int c = c0 + u * 256 + (lane >> 2) * 32;
         word[u] = 0;
         if (c >= p.cols) continue;
-        word[u] = __ldg(q0 + u * 32);
+        word[u] = q0[u * 32];
         s[u] = __half2float(p.scale[s0 + c / kGroup]);
         m[u] = kMin ? __half2float(p.min[s0 + c / kGroup]) : 0.0f;
     }
@@ -293,8 +294,8 @@ __global__ void __launch_bounds__(32 * kQ4Warps) dequantize_q4_kernel(const Conv
         if (!p.aligned) __syncwarp();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if (p.aligned) put4(w + c + 16 * h, left - c - 16 * h, true, v[h]);
-            else put4(line + c + 16 * h, 4, true, v[h]);
+            if (p.aligned) put4(w + c + 16 * h, left - c - 16 * h, v[h]);
+            else put4(line + c + 16 * h, 4, v[h]);
         }
         if (!p.aligned) { /* consecutive lanes, consecutive elements */
             __syncwarp();
@@ -371,7 +372,7 @@ __device__ __forceinline__ void stage_x(Dst dst, const int8_t *x, size_t step, i
 
 __device__ __forceinline__ void store_y(const MatvecParams &p, int b, int row, float v) {
     const size_t at = (size_t)b * p.y_stride + row;
-    v = __fmul_rn(__ldg(p.sx + b), v);
+    v = __fmul_rn(p.sx[b], v);
     if (p.dtype == LAL_TAIL_F32)
         ((float *)p.y)[at] = v;
     else if (p.dtype == LAL_TAIL_BF16)
@@ -394,7 +395,7 @@ __device__ __forceinline__ void store_tile_as(const MatvecParams &p, int b0, int
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             if (8 * n + 2 * t + c >= nx) break;
-            const float s = __ldg(sx + 8 * n + c);
+            const float s = sx[8 * n + c];
 #pragma unroll
             for (int r = 0; r < 2 * kMT; ++r)
                 if (g + 8 * r < rows)
@@ -431,9 +432,9 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
 
 /* How a warp's ring is filled.  kAligned: vectors and rows of scales begin at
  * 16-byte boundaries (scales: of a stage's size) and lie as ldmatrix wants
- * them.  kAny: the aligned 16-byte pieces around them are copied as they are,
- * and their offsets are taken at the reading, so these copies are asynchronous
- * too.  kMany (aligned, 32 rows a warp, tiles for several waves): more warps
+ * them.  kAny: the aligned 16-byte pieces around them are copied as they are
+ * (each holds a byte of its row, so none lies outside memory), and their
+ * offsets are taken at the reading, so these copies are asynchronous too.  kMany (aligned, 32 rows a warp, tiles for several waves): more warps
  * with shorter rings; 58 us against 68 for 152064x3584 g128 and sixteen streams,
  * but 30 against 17 for 37888x3584, one wave. */
 enum MmaFill { kAligned, kMany, kAny };
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
                     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(row + g0), "n"(2 * kGroups) : "memory");
                 } else {
 #pragma unroll
-                    for (int k = 0; k < kGroups; ++k) ((unsigned short *)to)[k] = g0 + k < groups ? __ldg(row + g0 + k) : 0;
+                    for (int k = 0; k < kGroups; ++k) ((unsigned short *)to)[k] = g0 + k < groups ? row[g0 + k] : 0;
                 }
             }
         };
@@ -712,13 +713,13 @@ cudaError_t launch_mma(const MatvecParams &p, int x_base, int num_sms, cudaStrea
  * 37888x3584 g128 with 64 streams 34.9 us, 0.33 of HBM's rate and 0.30 of the
  * bf16 one; bounded by the hand-overs between the warps' roles.
  *
- * A CTA takes tiles of 128 rows by up to kN streams.  The weights are the A
- * operand and lie in tensor memory: a thread of the four unpacking warps has a
+ * A CTA takes tiles of 128 rows by up to 64 streams.  The weights are the A
+ * operand and lie in tensor memory: a thread of the eight unpacking warps has a
  * row, reads its 16-byte blocks from a ring of its warp's own (cp.async) and
  * stores 16 (q - 8) as int8, eight columns of tensor memory a block.  The
  * vectors are the B operand, in shared memory with the 128-byte swizzle.  One
- * thread issues the products, a group of columns at a time into one of kD
- * accumulators; eight warps read a finished one (int32, exact), scale it by
+ * thread issues the products, a group of columns at a time into one of kTcD
+ * accumulators; sixteen warps read a finished one (int32, exact), scale it by
  * the row's scale of the group and add it in fp32 registers, while the next
  * groups are multiplied.  So every scale is applied in fp32, the weights are
  * read once, and only the unpacked weights' 8-bit form is ever written on the
@@ -745,10 +746,9 @@ struct TcShared {
     int abort, never;
 };
 
-__host__ __device__ constexpr int tc_x_stage(int n) { return n * kStageBlocks * 32; }
-__host__ __device__ constexpr int tc_sum_bytes(int n, int group) { return kTcXDepth * (kStageBlocks * 32 / group) * n * 4; }
-template <int kN, int kGroup, bool kMin> constexpr int tc_smem() {
-    return 1024 + kTcUnpack * kTcWDepth * kTcWStage + kTcXDepth * tc_x_stage(kN) + (kMin ? tc_sum_bytes(kN, kGroup) : 0);
+constexpr int kTcXStage = kTcStreams * kStageBlocks * 32;
+template <int kGroup, bool kMin> constexpr int tc_smem() {
+    return 1024 + kTcUnpack * kTcWDepth * kTcWStage + kTcXDepth * kTcXStage + (kMin ? kTcXDepth * (kStageBlocks * 32 / kGroup) * kTcStreams * 4 : 0);
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -779,35 +779,18 @@ __device__ __forceinline__ void tc_store8(uint32_t at, const uint32_t (&r)[8]) {
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
-template <int kCount> __device__ __forceinline__ void tc_load(uint32_t at, int (&r)[kCount]) {
-    if constexpr (kCount == 16)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-                     "%14, %15}, [%16];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                       "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                     : "r"(at));
-    else if constexpr (kCount == 8)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                     : "r"(at));
-    else
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                     : "r"(at));
+__device__ __forceinline__ void tc_load16(uint32_t at, int (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                 "%14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
     /* the wait names the registers, so that nothing reads them before it */
-    if constexpr (kCount == 16)
-        asm volatile("tcgen05.wait::ld.sync.aligned;"
-                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                       "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                     :
-                     : "memory");
-    else if constexpr (kCount == 8)
-        asm volatile("tcgen05.wait::ld.sync.aligned;"
-                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
-                     :
-                     : "memory");
-    else
-        asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]) : : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
 }
 
 /* A thread's results, n of kCount streams from b0, of a row. */
@@ -816,7 +799,7 @@ __device__ __forceinline__ void store_row(const MatvecParams &p, int b0, int n, 
     T *y = (T *)p.y + (size_t)b0 * p.y_stride + row;
 #pragma unroll
     for (int j = 0; j < kCount; ++j, y += p.y_stride)
-        if (j < n) *y = from_f32<T>(__fmul_rn(__ldg(p.sx + b0 + j), __fmul_rn(0.0625f, acc[j])));
+        if (j < n) *y = from_f32<T>(__fmul_rn(p.sx[b0 + j], __fmul_rn(0.0625f, acc[j])));
 }
 
 /* The stages of a CTA in order: every tile's range of K. */
@@ -843,15 +826,15 @@ __device__ __forceinline__ bool tc_wait(uint64_t *b, uint32_t parity, volatile i
     return true;
 }
 
-template <int kN, int kGroup, bool kMin>
+template <int kGroup, bool kMin>
 __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecParams p, int splits, int x_base) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ TcShared sh;
     constexpr int kPer = kGroup / kQ4Block, kGroups = kStageBlocks / kPer; /* blocks a group, groups a stage */
-    constexpr int kMine = kN / (kTcEpi / 4);                               /* streams of an epilogue warp */
+    constexpr int kN = kTcStreams, kMine = kN / (kTcEpi / 4);              /* streams of a tile, of an epilogue warp */
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t *xring = smem;                                      /* kTcXDepth stages of two swizzled tiles */
-    uint8_t *wring = xring + kTcXDepth * tc_x_stage(kN);        /* of each unpacking warp */
+    uint8_t *wring = xring + kTcXDepth * kTcXStage;        /* of each unpacking warp */
     float *xsums = (float *)(wring + kTcUnpack * kTcWDepth * kTcWStage); /* [kTcXDepth][kGroups][kN] */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *abort_flag = &sh.abort, *never = &sh.never;
@@ -969,13 +952,13 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                 const int row = min(ahead.tile * 128 + quad * 32 + lane, p.rows - 1), g0 = ahead.st * kGroups;
                 const size_t at = (size_t)row * groups + g0;
                 if (g0 + kGroups <= groups) {
-                    scale_next.all = __ldg((const Pack *)(p.scale + at));
-                    if (kMin) low_next.all = __ldg((const Pack *)(p.min + at));
+                    scale_next.all = *(const Pack *)(p.scale + at);
+                    if (kMin) low_next.all = *(const Pack *)(p.min + at);
                 } else {
 #pragma unroll
                     for (int i = 0; i < kGroups; ++i) {
-                        scale_next.one[i] = g0 + i < groups ? __ldg((const unsigned short *)p.scale + at + i) : 0;
-                        if (kMin) low_next.one[i] = g0 + i < groups ? __ldg((const unsigned short *)p.min + at + i) : 0;
+                        scale_next.one[i] = g0 + i < groups ? ((const unsigned short *)p.scale)[at + i] : 0;
+                        if (kMin) low_next.one[i] = g0 + i < groups ? ((const unsigned short *)p.min)[at + i] : 0;
                     }
                 }
             }
@@ -1003,7 +986,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                 }
                 tc_fence_after();
                 int c[kMine];
-                tc_load<kMine>(lanes + buf * kN, c);
+                tc_load16(lanes + buf * kN, c);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.d_empty[buf]);
@@ -1064,7 +1047,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                     break;
                 }
                 tc_fence_after();
-                const uint32_t xt = x0 + xs * (tc_x_stage(kN) >> 4);
+                const uint32_t xt = x0 + xs * (kTcXStage >> 4);
 #pragma unroll
                 for (int gr = 0; gr < kGroups; ++gr, ++d) {
                     const int acc_buf = d % kTcD;
@@ -1102,7 +1085,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             if (ahead.n < total) {
                 if (round > 0 && !tc_wait(&sh.x_empty[xs], (round & 1) ^ 1, abort_flag)) return false;
                 const int c0 = ahead.st * kStageBlocks * kQ4Block + (lane & 15) * 16;
-                uint8_t *dst = xring + xs * tc_x_stage(kN) + d0;
+                uint8_t *dst = xring + xs * kTcXStage + d0;
                 const int n = (nx - n0 + 2 * kTcLoad - 1) / (2 * kTcLoad); /* this lane's vectors, four at a time */
                 stage_x<4>([&](int j) { return dst + j * 1024; }, x0, x_step, min(n, 4), c0, p.cols);
                 if (n > 4)
@@ -1118,7 +1101,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             __syncwarp();
             if (kMin) {
                 /* 16 times the sum of each group of this warp's rows */
-                const uint8_t *st = xring + xs * tc_x_stage(kN);
+                const uint8_t *st = xring + xs * kTcXStage;
                 for (int i = lane; i < kN / kTcLoad * kGroups; i += 32) {
                     const int gr = i % kGroups, pair = i / kGroups;
                     const int n = (pair >> 1) * 2 * kTcLoad + lw * 2 + (pair & 1);
@@ -1189,16 +1172,15 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
 
 template <int kGroup, bool kMin>
 cudaError_t launch_tc(const MatvecParams &p, int x_base, int chunks, int num_sms, cudaStream_t st) {
-    constexpr int kN = kTcStreams;
     const int tiles = (p.rows + 127) / 128, stages = (q4_blocks(p.cols) + kStageBlocks - 1) / kStageBlocks;
     /* CTAs of a tile: as many as leave each an SM and two stages */
     int splits = 1;
     while (splits < kTcMaxSplit && (long long)tiles * chunks * splits * 2 <= num_sms && splits * 4 <= stages) splits *= 2;
-    const void *fn = (const void *)q4_tc_kernel<kN, kGroup, kMin>;
-    constexpr int smem = tc_smem<kN, kGroup, kMin>();
+    const void *fn = (const void *)q4_tc_kernel<kGroup, kMin>;
+    constexpr int smem = tc_smem<kGroup, kMin>();
     cudaError_t e = raise_smem(fn, smem);
     if (e != cudaSuccess) return e;
-    return launch_early(q4_tc_kernel<kN, kGroup, kMin>,
+    return launch_early(q4_tc_kernel<kGroup, kMin>,
                         dim3((unsigned)(splits > 1 ? tiles * splits : std::min(tiles, num_sms)), (unsigned)chunks), 32 * kTcWarps,
                         smem, st, splits, p, splits, x_base);
 }
@@ -1290,7 +1272,7 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
                     } else {
 #pragma unroll
                         for (int k = 0; k < kGroups; ++k) {
-                            const unsigned short v = g0 + k < groups ? __ldg(src + k) : 0;
+                            const unsigned short v = g0 + k < groups ? src[k] : 0;
                             asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + 2 * k), "h"(v) : "memory");
                         }
                     }
@@ -1325,7 +1307,7 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
         if (row0 < end) {
             /* blocks behind the row's end hold zeros in the vectors, and their groups scales of zero */
             const uint32_t at = slot * Stage::kW, xt = slot * Stage::kX;
-#pragma unroll(kNT <= 2 ? kUnits : 1)
+#pragma unroll 1
             for (int u = 0; u < kUnits; ++u) {
                 uint32_t a[kMT][kUnit][4];
 #pragma unroll
@@ -1364,7 +1346,7 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
                         }
                     }
                 /* kB eights of vectors at once: as many independent products again */
-                constexpr int kB = kNT < 2 ? 1 : 2;
+                constexpr int kB = 2;
 #pragma unroll
                 for (int n0 = 0; n0 < kNT; n0 += kB) {
                     uint32_t x[kB][kUnit / 2][4];

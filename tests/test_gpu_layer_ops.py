@@ -687,3 +687,132 @@ def test_matvec_many_rows(streams, rows, cols):
     rng = np.random.default_rng(rows)
     check_matvec(rng, streams, rows, cols, 32, True, "bf16", 0)
     check_matvec(rng, streams, rows, cols, 128, False, "f32", 3)
+
+
+@pytest.mark.parametrize("streams,cols", [(1, 1024), (3, 1003), (16, 1024), (20, 1003), (32, 1024), (64, 1024)])
+def test_a_call_sees_what_the_call_before_it_wrote(streams, cols):
+    """Calls follow each other with nothing between them, and each reads what
+    the one before has just written over: sums in place, 8-bit rows, weights
+    and their scales.  As when every call is waited for."""
+    rows, rounds = 20000, 6
+    rng = np.random.default_rng(3)
+    w = Weights(rows, cols, 32, True)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    full = [torch.randn(rows, cols, generator=g, device="cuda") * (1 + k) for k in range(rounds)]
+    r = [torch.randn(streams, cols, generator=g, device="cuda").to(torch.bfloat16) for _ in range(rounds)]
+    norm_w = torch.as_tensor(1 + 0.1 * rng.standard_normal(cols), dtype=torch.float32).cuda()
+    runs = []
+    for wait in (True, False):
+        h = torch.zeros(streams, cols, dtype=torch.bfloat16, device="cuda")
+        q = torch.zeros(streams, cols, dtype=torch.int8, device="cuda")
+        s = torch.zeros(streams, device="cuda")
+        y = torch.zeros(rounds, streams, rows, device="cuda")
+        torch.cuda.synchronize()
+        for k in range(rounds):
+            calls = [lambda k=k, j=j: L.add_rms_norm_q8(
+                h.data_ptr(), r[(k + j) % rounds].data_ptr(), h.data_ptr(), norm_w.data_ptr(), 1e-6, streams, cols,
+                q.data_ptr(), s.data_ptr(), L.LAL_TAIL_BF16, stream=stream()) for j in range(3)]
+            calls.insert(1, lambda k=k: w.w.quantize(full[k].data_ptr(), stream=stream()))
+            if k % 2:  # the norm, or the quantizer, directly before the product
+                calls = calls[:1] + calls[2:] + calls[1:2]
+            calls.append(lambda k=k: w.w.matvec(q.data_ptr(), s.data_ptr(), streams, y[k].data_ptr(), stream=stream()))
+            for call in calls:
+                call()
+                if wait:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        runs.append((h.clone(), q.clone(), s.clone(), y))
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+    assert all(bool((runs[0][3][k] != runs[0][3][k - 1]).any()) for k in range(1, rounds))
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("streams", [2, 24, 64])
+def test_products_on_two_streams_joined(streams, captured):
+    """Gate and up at once on two streams behind one norm, joined at the
+    SwiGLU; copies and a memset are what the operators follow and precede."""
+    d, f = 1024, 2048
+    x = activations(np.random.default_rng(1), streams, d)
+    x_host = torch.as_tensor(x, dtype=torch.float32).pin_memory()
+    weights = [Weights(f, d, 64, False) for _ in range(2)]
+    for k, w in enumerate(weights):
+        full = torch.randn(f, d, generator=torch.Generator().manual_seed(k)).cuda()
+        w.w.quantize(full.data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+    norm_w = torch.ones(d, device="cuda")
+    dx, y = torch.empty(streams, d, device="cuda"), torch.empty(2, streams, f, device="cuda")
+    q, aq = (torch.empty(streams, n, dtype=torch.int8, device="cuda") for n in (d, f))
+    s, asc, out = torch.empty(streams, device="cuda"), torch.empty(streams, device="cuda"), torch.empty_like(aq)
+    side, main = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def run():
+        here = torch.cuda.current_stream()
+        dx.copy_(x_host, non_blocking=True)
+        L.add_rms_norm_q8(dx.data_ptr(), None, None, norm_w.data_ptr(), 1e-6, streams, d, q.data_ptr(), s.data_ptr(),
+                          stream=here.cuda_stream)
+        side.wait_stream(here)
+        weights[0].w.matvec(q.data_ptr(), s.data_ptr(), streams, y[0].data_ptr(), stream=here.cuda_stream)
+        weights[1].w.matvec(q.data_ptr(), s.data_ptr(), streams, y[1].data_ptr(), stream=side.cuda_stream)
+        here.wait_stream(side)
+        L.swiglu_q8(y[0].data_ptr(), y[1].data_ptr(), streams, f, aq.data_ptr(), asc.data_ptr(), stream=here.cuda_stream)
+        out.copy_(aq, non_blocking=True)
+        y.zero_()
+
+    with torch.cuda.stream(main):
+        if captured:
+            run()  # (a first run outside)
+            torch.cuda.synchronize()
+            out.zero_(), asc.zero_()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=main):
+                run()
+            for _ in range(4):
+                graph.replay()
+        else:
+            for _ in range(4):
+                run()
+    torch.cuda.synchronize()
+    # one call after another
+    want = torch.empty_like(y)
+    L.add_rms_norm_q8(dx.data_ptr(), None, None, norm_w.data_ptr(), 1e-6, streams, d, q.data_ptr(), s.data_ptr(), stream=stream())
+    for k in range(2):
+        weights[k].w.matvec(q.data_ptr(), s.data_ptr(), streams, want[k].data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+    wq, ws = ref.swiglu_q8(f64(want[0]), f64(want[1]))
+    check_rows(out, asc, wq, ws)
+    assert bool((y == 0).all())
+
+
+@pytest.mark.parametrize("streams", [12, 64])
+def test_block_into_the_batched_tail_without_waiting(streams):
+    """Blocks and batched steps one behind the other on the tail's stream give
+    the tokens that they give when each is waited for."""
+    cfg = synth.CONFIGS["c1_gpt2"].with_(vocab=5003, n_embd=1024, hist=16)
+    b = Block(streams, 1024, 1536, 32, "f32")
+    rng = np.random.default_rng(1)
+    w = (1.0 + 0.2 * rng.standard_normal(cfg.n_embd)).astype(np.float32)
+    u = torch.rand(8, streams, generator=torch.Generator().manual_seed(2)).cuda()
+    tokens = []
+    for wait in (True, False):
+        t = L.DecodeTail(cfg.vocab, cfg.n_embd, max_top_k=cfg.top_k, history_cap=cfg.hist,
+                         max_streams=streams)
+        t.load_lm_head_f32(synth.lm_head_f32(cfg))
+        t.set_sampling([cfg.temperature] * streams, [cfg.top_k] * streams, [cfg.rep_penalty] * streams)
+        for k in range(streams):
+            t.set_history(k, synth.history(cfg, k))
+        t.set_final_norm(w, 1e-6)
+        tok = torch.empty(8, streams, dtype=torch.int32, device="cuda")
+        b.feed(4)
+        torch.cuda.synchronize()
+        for step in range(8):
+            b.run(t.stream())
+            t.step_device(b.h.data_ptr(), streams, u[step].data_ptr(), tok[step].data_ptr())
+            if wait:
+                t.sync()
+        t.sync()
+        tokens.append(tok.cpu())
+        t.close()
+    assert torch.equal(tokens[0], tokens[1])
+    assert len(torch.unique(tokens[0])) > 1
