@@ -718,8 +718,8 @@ cudaError_t launch_mma(const MatvecParams &p, int x_base, int num_sms, cudaStrea
  * row, reads its 16-byte blocks from a ring of its warp's own (cp.async) and
  * stores 16 (q - 8) as int8, eight columns of tensor memory a block.  The
  * vectors are the B operand, in shared memory with the 128-byte swizzle.  One
- * thread issues the products, a group of columns at a time into one of kTcD
- * accumulators; sixteen warps read a finished one (int32, exact), scale it by
+ * thread issues the products, two groups of columns at a time into two of kTcD
+ * accumulators; sixteen warps read finished ones (int32, exact), scale it by
  * the row's scale of the group and add it in fp32 registers, while the next
  * groups are multiplied.  So every scale is applied in fp32, the weights are
  * read once, and only the unpacked weights' 8-bit form is ever written on the
@@ -732,7 +732,8 @@ constexpr int kTcUnpack = 8, kTcEpi = 16, kTcLoad = 4;
 constexpr int kTcIssue = kTcUnpack + kTcEpi; /* the warp that issues the products */
 constexpr int kTcWarps = kTcIssue + 1 + kTcLoad;
 constexpr int kTcA = 4;        /* stages of unpacked weights in tensor memory, 64 columns each */
-constexpr int kTcD = 4;        /* accumulators */
+constexpr int kTcD = 4;        /* accumulators, handed over in pairs: half as many waits and commits as one by one */
+constexpr int kTcPairs = kTcD / 2;
 constexpr int kTcWDepth = 6;   /* stages of a warp's weight ring */
 constexpr int kTcXDepth = 4;   /* stages of the vectors */
 constexpr int kTcHalf = kStageBlocks / 2;         /* blocks of a stage that an unpacking warp has */
@@ -741,14 +742,16 @@ constexpr int kTcMaxSplit = 8;
 constexpr int kTcStreams = 64;
 
 struct TcShared {
-    uint64_t a_full[kTcA], a_empty[kTcA], x_full[kTcXDepth], x_empty[kTcXDepth], d_full[kTcD], d_empty[kTcD], drain;
+    uint64_t a_full[kTcA], a_empty[kTcA], x_full[kTcXDepth], x_empty[kTcXDepth], d_full[kTcPairs], d_empty[kTcPairs], drain;
     uint32_t tmem;
     int abort, never;
 };
 
 constexpr int kTcXStage = kTcStreams * kStageBlocks * 32;
 template <int kGroup, bool kMin> constexpr int tc_smem() {
-    return 1024 + kTcUnpack * kTcWDepth * kTcWStage + kTcXDepth * kTcXStage + (kMin ? kTcXDepth * (kStageBlocks * 32 / kGroup) * kTcStreams * 4 : 0);
+    constexpr int kGroups = kStageBlocks * kQ4Block / kGroup; /* of a stage: scales (and minima), sums of the vectors */
+    return 1024 + kTcUnpack * kTcWDepth * kTcWStage +
+           kTcXDepth * (kTcXStage + 128 * kGroups * (kMin ? 4 : 2) + (kMin ? kGroups * kTcStreams * 4 : 0));
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -835,7 +838,8 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t *xring = smem;                                      /* kTcXDepth stages of two swizzled tiles */
     uint8_t *wring = xring + kTcXDepth * kTcXStage;        /* of each unpacking warp */
-    float *xsums = (float *)(wring + kTcUnpack * kTcWDepth * kTcWStage); /* [kTcXDepth][kGroups][kN] */
+    uint8_t *sring = wring + kTcUnpack * kTcWDepth * kTcWStage; /* scales: [kTcXDepth][1, or 2 with minima][128][kGroups] */
+    float *xsums = (float *)(sring + kTcXDepth * 128 * kGroups * (kMin ? 4 : 2)); /* [kTcXDepth][kGroups][kN] */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *abort_flag = &sh.abort, *never = &sh.never;
     const int b0 = x_base + blockIdx.y * kN, nx = min(kN, p.streams - b0);
@@ -851,8 +855,8 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
     if (threadIdx.x == 0) {
         for (int i = 0; i < kTcA; ++i) mbar_init(&sh.a_full[i], kTcUnpack), mbar_init(&sh.a_empty[i], 1);
         for (int i = 0; i < kTcXDepth; ++i)
-            mbar_init(&sh.x_full[i], kTcLoad), mbar_init(&sh.x_empty[i], 1 + (kMin ? kTcEpi : 0));
-        for (int i = 0; i < kTcD; ++i) mbar_init(&sh.d_full[i], 1), mbar_init(&sh.d_empty[i], kTcEpi);
+            mbar_init(&sh.x_full[i], kTcLoad), mbar_init(&sh.x_empty[i], kTcEpi);
+        for (int i = 0; i < kTcPairs; ++i) mbar_init(&sh.d_full[i], 1), mbar_init(&sh.d_empty[i], kTcEpi);
         mbar_init(&sh.drain, 1);
         sh.abort = sh.never = 0;
         mbar_fence_init();
@@ -945,73 +949,59 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             Pack all;
             unsigned short one[kGroups];
             __device__ Row() {}
-        } scale, low, scale_next, low_next;
-        TcWalk ahead(tile0, st0);
-        auto load_scales = [&] {
-            if (ahead.n < total) {
-                const int row = min(ahead.tile * 128 + quad * 32 + lane, p.rows - 1), g0 = ahead.st * kGroups;
-                const size_t at = (size_t)row * groups + g0;
-                if (g0 + kGroups <= groups) {
-                    scale_next.all = *(const Pack *)(p.scale + at);
-                    if (kMin) low_next.all = *(const Pack *)(p.min + at);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kGroups; ++i) {
-                        scale_next.one[i] = g0 + i < groups ? ((const unsigned short *)p.scale)[at + i] : 0;
-                        if (kMin) low_next.one[i] = g0 + i < groups ? ((const unsigned short *)p.min)[at + i] : 0;
-                    }
-                }
-            }
-            ahead.next(st0, st1, tile_step);
-        };
-        load_scales();
+        } scale, low;
         bool ok = true;
         TcWalk at(tile0, st0);
         for (int d = 0, xs = 0, xs_round = 0; at.n < total; at.next(st0, st1, tile_step)) {
             if (at.st == st0)
 #pragma unroll
                 for (int j = 0; j < kMine; ++j) acc[j] = 0.0f;
-            scale.all = scale_next.all;
-            if (kMin) low.all = low_next.all;
-            load_scales();
-            if (kMin && !tc_wait(&sh.x_full[xs], xs_round & 1, abort_flag)) ok = false;
+            if (!tc_wait(&sh.x_full[xs], xs_round & 1, abort_flag)) ok = false;
+            const Pack *sc = (const Pack *)sring + xs * (kMin ? 256 : 128) + quad * 32 + lane;
+            scale.all = sc[0];
+            if (kMin) low.all = sc[128];
 #pragma unroll
-            for (int gr = 0; gr < kGroups; ++gr, ++d) {
-                const int buf = d % kTcD;
-                if (ok && !tc_wait(&sh.d_full[buf], (d / kTcD) & 1, abort_flag)) ok = false;
+            for (int pair = 0; pair < kGroups / 2; ++pair, ++d) {
+                const int buf = d % kTcPairs;
+                if (ok && !tc_wait(&sh.d_full[buf], (d / kTcPairs) & 1, abort_flag)) ok = false;
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     *abort_flag = 1;
                     break;
                 }
                 tc_fence_after();
-                int c[kMine];
-                tc_load16(lanes + buf * kN, c);
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.d_empty[buf]);
-                const float s = __half2float(__ushort_as_half(scale.one[gr]));
 #pragma unroll
-                for (int j = 0; j < kMine; ++j) acc[j] = fmaf(s, (float)c[j], acc[j]);
-                if (kMin) {
-                    const float m = fmaf(8.0f, s, __half2float(__ushort_as_half(low.one[gr])));
-                    const float4 *sum = (const float4 *)(xsums + (xs * kGroups + gr) * kN + part * kMine);
+                for (int h = 0; h < 2; ++h) {
+                    const int gr = 2 * pair + h;
+                    int c[kMine];
+                    tc_load16(lanes + (2 * buf + h) * kN, c);
+                    if (h == 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.d_empty[buf]);
+                    }
+                    const float s = __half2float(__ushort_as_half(scale.one[gr]));
 #pragma unroll
-                    for (int j = 0; j < kMine; j += 4) {
-                        const float4 v = sum[j / 4];
-                        acc[j] = fmaf(m, v.x, acc[j]);
-                        acc[j + 1] = fmaf(m, v.y, acc[j + 1]);
-                        acc[j + 2] = fmaf(m, v.z, acc[j + 2]);
-                        acc[j + 3] = fmaf(m, v.w, acc[j + 3]);
+                    for (int j = 0; j < kMine; ++j) acc[j] = fmaf(s, (float)c[j], acc[j]);
+                    if (kMin) {
+                        const float m = fmaf(8.0f, s, __half2float(__ushort_as_half(low.one[gr])));
+                        const float4 *sum = (const float4 *)(xsums + (xs * kGroups + gr) * kN + part * kMine);
+#pragma unroll
+                        for (int j = 0; j < kMine; j += 4) {
+                            const float4 v = sum[j / 4];
+                            acc[j] = fmaf(m, v.x, acc[j]);
+                            acc[j + 1] = fmaf(m, v.y, acc[j + 1]);
+                            acc[j + 2] = fmaf(m, v.z, acc[j + 2]);
+                            acc[j + 3] = fmaf(m, v.w, acc[j + 3]);
+                        }
                     }
                 }
             }
             if (!ok) break;
-            if (kMin) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.x_empty[xs]);
-                if (++xs == kTcXDepth) xs = 0, ++xs_round;
-            }
+            /* the stage's products are complete, its vectors and scales read */
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.x_empty[xs]);
+            if (++xs == kTcXDepth) xs = 0, ++xs_round;
             if (splits == 1 && at.st == st1 - 1) {
                 const int row = at.tile * 128 + quad * 32 + lane;
                 if (row < p.rows) {
@@ -1049,22 +1039,21 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                 tc_fence_after();
                 const uint32_t xt = x0 + xs * (kTcXStage >> 4);
 #pragma unroll
-                for (int gr = 0; gr < kGroups; ++gr, ++d) {
-                    const int acc_buf = d % kTcD;
-                    if (d >= kTcD && !tc_wait(&sh.d_empty[acc_buf], ((d / kTcD) & 1) ^ 1, abort_flag)) {
+                for (int pair = 0; pair < kGroups / 2; ++pair, ++d) {
+                    const int d_buf = d % kTcPairs;
+                    if (d >= kTcPairs && !tc_wait(&sh.d_empty[d_buf], ((d / kTcPairs) & 1) ^ 1, abort_flag)) {
                         *abort_flag = 1;
                         ok = false;
                         break;
                     }
                     tc_fence_after();
 #pragma unroll
-                    for (int k = gr * kPer; k < (gr + 1) * kPer; ++k)
-                        tc_mma_i8_ta(tmem_d + acc_buf * kN, tmem + buf * 64 + k * 8, xt + (k / 4) * (kN * 128 >> 4) + (k % 4) * 2,
-                                     tc_idesc(kN), k != gr * kPer);
-                    tc_commit(&sh.d_full[acc_buf]);
+                    for (int k = 2 * pair * kPer; k < 2 * (pair + 1) * kPer; ++k)
+                        tc_mma_i8_ta(tmem_d + (2 * d_buf + k / kPer % 2) * kN, tmem + buf * 64 + k * 8,
+                                     xt + (k / 4) * (kN * 128 >> 4) + (k % 4) * 2, tc_idesc(kN), k % kPer != 0);
+                    tc_commit(&sh.d_full[d_buf]);
                 }
                 tc_commit(&sh.a_empty[buf]);
-                tc_commit(&sh.x_empty[xs]);
                 if (++xs == kTcXDepth) xs = 0, ++xs_round;
             }
             /* every product issued is complete before the tensor memory is freed */
@@ -1072,7 +1061,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             if (!tc_wait(&sh.drain, 0u, never)) *abort_flag = 1;
         }
     } else {
-        /* ---- vectors, and (with minima) their sums ---- */
+        /* ---- vectors, and (with minima) their sums; scales ---- */
         const int lw = warp - kTcIssue - 1;
         /* a loader warp has every kTcLoad-th pair of rows: 16 lanes a row */
         const int n0 = lw * 2 + (lane >> 4);
@@ -1090,6 +1079,19 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                 stage_x<4>([&](int j) { return dst + j * 1024; }, x0, x_step, min(n, 4), c0, p.cols);
                 if (n > 4)
                     stage_x<4>([&](int j) { return dst + 4096 + j * 1024; }, x0 + 4 * x_step, x_step, n - 4, c0, p.cols);
+                /* the scales of row 32 lw + lane: as many stages ahead, their latency is HBM's */
+                const int row = min(ahead.tile * 128 + lw * 32 + lane, p.rows - 1), g0 = ahead.st * kGroups;
+#pragma unroll
+                for (int m = 0; m < (kMin ? 2 : 1); ++m) {
+                    const unsigned short *src = (const unsigned short *)(m ? p.min : p.scale) + (size_t)row * groups + g0;
+                    uint8_t *to = sring + ((xs * (kMin ? 2 : 1) + m) * 128 + lw * 32 + lane) * (2 * kGroups);
+                    if (g0 + kGroups <= groups) {
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(src), "n"(2 * kGroups) : "memory");
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < kGroups; ++k) ((unsigned short *)to)[k] = g0 + k < groups ? src[k] : 0;
+                    }
+                }
             }
             ahead.next(st0, st1, tile_step);
             cp_async_commit();
