@@ -710,8 +710,9 @@ cudaError_t launch_mma(const MatvecParams &p, int x_base, int num_sms, cudaStrea
 
 /* ---- 33 streams and more: tcgen05.mma kind::i8 ----
  *
- * 37888x3584 g128 with 64 streams 34.9 us, 0.33 of HBM's rate and 0.30 of the
- * bf16 one; bounded by the hand-overs between the warps' roles.
+ * 37888x3584 g128 with 64 streams 30.5 us, 0.38 of HBM's rate and 0.34 of the
+ * bf16 one; bounded by what the warps' roles take in turn a stage (with their
+ * arithmetic, products and vectors taken out it still takes 21 us).
  *
  * A CTA takes tiles of 128 rows by up to 64 streams.  The weights are the A
  * operand and lie in tensor memory: a thread of the eight unpacking warps has a
@@ -719,9 +720,9 @@ cudaError_t launch_mma(const MatvecParams &p, int x_base, int num_sms, cudaStrea
  * stores 16 (q - 8) as int8, eight columns of tensor memory a block.  The
  * vectors are the B operand, in shared memory with the 128-byte swizzle.  One
  * thread issues the products, two groups of columns at a time into two of kTcD
- * accumulators; sixteen warps read finished ones (int32, exact), scale it by
- * the row's scale of the group and add it in fp32 registers, while the next
- * groups are multiplied.  So every scale is applied in fp32, the weights are
+ * accumulators; sixteen warps read finished ones (int32, exact), scale them
+ * by the row's scales of the groups and add them in fp32 registers, while the
+ * next groups are multiplied.  So every scale is applied in fp32, the weights are
  * read once, and only the unpacked weights' 8-bit form is ever written on the
  * chip.  With few tiles, the K range of a tile is split over a cluster of
  * CTAs, whose sums are exchanged and added in order over distributed shared
@@ -732,7 +733,7 @@ constexpr int kTcUnpack = 8, kTcEpi = 16, kTcLoad = 4;
 constexpr int kTcIssue = kTcUnpack + kTcEpi; /* the warp that issues the products */
 constexpr int kTcWarps = kTcIssue + 1 + kTcLoad;
 constexpr int kTcA = 4;        /* stages of unpacked weights in tensor memory, 64 columns each */
-constexpr int kTcD = 4;        /* accumulators, handed over in pairs: half as many waits and commits as one by one */
+constexpr int kTcD = 4;        /* accumulators, handed over in pairs: 30.6 us against 35.1 one by one, groups of 32 53.6 against 69.8 */
 constexpr int kTcPairs = kTcD / 2;
 constexpr int kTcWDepth = 6;   /* stages of a warp's weight ring */
 constexpr int kTcXDepth = 4;   /* stages of the vectors */
@@ -1429,14 +1430,14 @@ inline bool all_aligned(const MatvecParams &p) {
 /* Which kernel for the last (at most 64) streams, from x_base on.  Measured on a
  * B200, back to back, us:
  *   streams  weights            mma    shared vectors  tcgen05
- *   16       152064x3584 g128   58     97              135
- *   16       37888x3584  g32    25.2   29.2            69.5
- *   32       37888x3584  g128   29.0   22.3            34.1
- *   32       37888x3584  g32    46.0   29.8            69.6
- *   32       3584x3584   g32    10.5   26.8            16.1
- *   64       37888x3584  g128   56.7                   34.9
- *   64       37888x3584  g32    85.8                   70.5
- *   64       3584x3584   g32    19.5                   16.6
+ *   16       152064x3584 g128   58     97              115
+ *   16       37888x3584  g32    25.2   29.2            53.0
+ *   32       37888x3584  g128   29.0   22.3            29.7
+ *   32       37888x3584  g32    46.0   29.8            53.0
+ *   32       3584x3584   g32    10.5   26.8            13.9
+ *   64       37888x3584  g128   56.7                   30.4
+ *   64       37888x3584  g32    85.8                   53.5
+ *   64       3584x3584   g32    19.5                   14.4
  * so mma up to 16 streams, shared vectors up to 32 where every SM has 128
  * rows, tcgen05 beyond (and for whole 64s).  What is not aligned takes mma, 16
  * streams at a time. */
