@@ -232,7 +232,10 @@ template <typename T, bool kWide_> struct SwigluRow {
             asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
             e = fmaf(__fmul_rn(e, lo), kLn2, e);
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, e)));
-            v[j] = __fmul_rn(__fmul_rn(v[j], r), up[j]);
+            /* gate * up first: where that is subnormal v is too, far below any row's step, while gate * r
+             * may be subnormal and v large.  Gates above 2.36e38 give NaN (hi overflows), products that
+             * overflow infinity: such rows find their maximum, and store() such elements, in 64 bits. */
+            v[j] = __fmul_rn(__fmul_rn(v[j], up[j]), r);
         }
     }
     __device__ void again(int i, float (&v)[8]) const {
@@ -366,7 +369,7 @@ template <typename Row> struct RowQuant {
         for (int j = 0; j < 8; ++j) {
             const float t = __fmul_rn(v[j], r32);
             u[j] = __fadd_rn(t, kRound);
-            far = fmaxf(far, off_centre(t, u[j]));
+            far = max_nan(far, off_centre(t, u[j])); /* a v that 32 bits do not have goes to 64 */
         }
         uint32_t w[2];
 #pragma unroll
