@@ -334,7 +334,8 @@ cudaError_t prepare_sample_kernel();
 cudaError_t launch_sample_prepared(const TailParams &p, int grid, cudaStream_t st);
 /* Records the calling thread's last error message (tail_api.cu). */
 int set_error(int code, const char *msg);
-/* Raise a kernel's dynamic shared-memory limit once per (device, kernel). */
+/* Raise a kernel's dynamic shared-memory limit on the current device to at
+ * least `bytes` (never lowered, whichever thread asks). */
 cudaError_t raise_smem(const void *fn, int bytes);
 
 /* Batched step (tail_batch.cu): B >= 2 streams share one pass over W on the

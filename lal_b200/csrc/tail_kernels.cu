@@ -36,6 +36,7 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
+#include <mutex>
 #include <numeric>
 #include <utility>
 #include <vector>
@@ -2150,17 +2151,42 @@ int plan_launch(TailParams &p, int num_sms, int min_rows_per_cta) {
     return G;
 }
 
-/* Raise a kernel's dynamic shared-memory limit once per (device, kernel). */
+/* Raise a kernel's dynamic shared-memory limit on the current device to at
+ * least `bytes`.  The limit belongs to the process: what any thread's launch
+ * needs stays, so it is only ever raised.  A thread remembers the limits that
+ * it has seen, and takes the lock for a larger one alone. */
 cudaError_t raise_smem(const void *fn, int bytes) {
-    thread_local std::vector<std::pair<int, const void *>> raised;
+    struct Limit {
+        int dev;
+        const void *fn;
+        int bytes;
+    };
+    static std::mutex lock;
+    static std::vector<Limit> limits;
+    thread_local std::vector<Limit> seen;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    for (const auto &r : raised)
-        if (r.first == dev && r.second == fn) return cudaSuccess;
-    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return e;
-    raised.emplace_back(dev, fn);
+    auto find = [&](std::vector<Limit> &in) -> Limit & {
+        for (Limit &l : in)
+            if (l.dev == dev && l.fn == fn) return l;
+        in.push_back({dev, fn, 0});
+        return in.back();
+    };
+    try {
+        Limit &mine = find(seen);
+        if (mine.bytes >= bytes) return cudaSuccess;
+        std::lock_guard<std::mutex> held(lock);
+        Limit &all = find(limits);
+        if (all.bytes < bytes) {
+            e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (e != cudaSuccess) return e;
+            all.bytes = bytes;
+        }
+        mine.bytes = all.bytes;
+    } catch (...) { /* no memory for the lists, or no lock */
+        return cudaErrorMemoryAllocation;
+    }
     return cudaSuccess;
 }
 
