@@ -365,7 +365,9 @@ __global__ void __launch_bounds__(NT, 1) tail_kernel(const __grid_constant__ Tai
         const int ctid = tid; /* 0 .. kConsumerWarps*32-1 */
         constexpr int NC = kConsumerWarps * 32;
         /* every global load of the prologue is issued before any result is
-         * used: hidden values and history ids into registers, scales to smem */
+         * used: hidden values and history ids into registers, scales to smem.
+         * The hidden vector is what the kernel before wrote, maybe while this
+         * one was already resident: not a read-only load (ld.global.nc) */
         constexpr int kHReg = 16;
         const float *h = p.hidden;
         float hv[kHReg];
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(NT, 1) tail_kernel(const __grid_constant__ Tai
 #pragma unroll
             for (int j = 0; j < kHReg; ++j) {
                 const int i = ctid + j * NC;
-                hv[j] = i < p.d ? __ldg(h + i) : 0.0f;
+                hv[j] = i < p.d ? __ldcg(h + i) : 0.0f;
             }
         }
         if (MODE != MODE_LMHEAD) {
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(NT, 1) tail_kernel(const __grid_constant__ Tai
         if (qin) {
 #pragma unroll
             for (int j = 0; j < kHReg; ++j) m = fmaxf(m, fabsf(hv[j]));
-            for (int i = ctid + kHReg * NC; i < p.d; i += NC) m = fmaxf(m, fabsf(__ldg(h + i)));
+            for (int i = ctid + kHReg * NC; i < p.d; i += NC) m = fmaxf(m, fabsf(__ldcg(h + i)));
         }
         m = consumer_max_f(m, ms); /* also orders the zeroing before the adds */
         if (ctid == 0) stamp(p, cta * 8 + 6); /* the hidden vector's maximum */
@@ -500,7 +502,7 @@ __global__ void __launch_bounds__(NT, 1) tail_kernel(const __grid_constant__ Tai
                     if (i < p.ld) xq_s[i] = quant(i, hv[j]);
                 }
                 for (int i = ctid + kHReg * NC; i < p.ld; i += NC)
-                    xq_s[i] = quant(i, i < p.d ? __ldg(h + i) : 0.0f);
+                    xq_s[i] = quant(i, i < p.d ? __ldcg(h + i) : 0.0f);
             }
             if (ctid == 0) ms->sx = scale;
         } else if (MODE == MODE_LMHEAD) {

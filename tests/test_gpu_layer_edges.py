@@ -4,11 +4,13 @@ tolerances are that file's."""
 import numpy as np
 import pytest
 
+import lal_b200 as L
+from lal_b200 import synth
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_layer_ops import check_rows, run_swiglu  # noqa: E402
+from test_gpu_layer_ops import Weights, check_rows, run_swiglu, stream  # noqa: E402
 
 
 # ---- SwiGLU at gates that 32-bit intermediates do not hold --------------------------------
@@ -43,3 +45,84 @@ def test_swiglu_extreme_gates(dtype, rows, n, pad):
     q, s, want = run_swiglu(g, u, dtype, pad)
     assert np.isfinite(want[1]).all() and (want[1] > 0).all()
     check_rows(q, s, *want)
+
+
+# ---- the chain into the one-stream tail ---------------------------------------------------
+
+class MixedBlock:
+    """An MLP block whose residual stream is fp32, as the tail's hidden vectors
+    are, and whose gate and up are bf16; h and y run on from step to step."""
+
+    def __init__(self, streams, d, f, group, seed=0):
+        rng = np.random.default_rng(seed)
+        self.n, self.d, self.f = streams, d, f
+        self.gate_up, self.down = Weights(2 * f, d, group, False), Weights(d, f, group, True)
+        for w, r, c in ((self.gate_up, 2 * f, d), (self.down, d, f)):
+            full = torch.as_tensor(rng.standard_normal((r, c)) / np.sqrt(c), dtype=torch.float32).cuda()
+            w.w.quantize(full.data_ptr(), L.LAL_TAIL_F32, stream=stream())
+            torch.cuda.synchronize()
+        self.norm_w = torch.as_tensor(1 + 0.1 * rng.standard_normal(d), dtype=torch.float32).cuda()
+        self.start = torch.as_tensor(rng.standard_normal((2, streams, d)), dtype=torch.float32).cuda()
+        self.h, self.y = torch.empty_like(self.start[0]), torch.empty_like(self.start[0])
+        self.gu = torch.empty(streams, 2 * f, dtype=torch.bfloat16, device="cuda")
+        self.q, self.aq = (torch.empty(streams, k, dtype=torch.int8, device="cuda") for k in (d, f))
+        self.s, self.asc = (torch.empty(streams, device="cuda") for _ in range(2))
+
+    def reset(self):
+        self.h.copy_(self.start[0])
+        self.y.copy_(self.start[1])
+
+    def calls(self, st):
+        n, d, f = self.n, self.d, self.f
+        return [
+            lambda: L.add_rms_norm_q8(self.y.data_ptr(), self.h.data_ptr(), self.h.data_ptr(), self.norm_w.data_ptr(), 1e-6,
+                                      n, d, self.q.data_ptr(), self.s.data_ptr(), L.LAL_TAIL_F32, stream=st),
+            lambda: self.gate_up.w.matvec(self.q.data_ptr(), self.s.data_ptr(), n, self.gu.data_ptr(), L.LAL_TAIL_BF16, stream=st),
+            lambda: L.swiglu_q8(self.gu.data_ptr(), self.gu.data_ptr() + 2 * f, n, f, self.aq.data_ptr(), self.asc.data_ptr(),
+                                L.LAL_TAIL_BF16, gate_stride=2 * f, up_stride=2 * f, stream=st),
+            lambda: self.down.w.matvec(self.aq.data_ptr(), self.asc.data_ptr(), n, self.y.data_ptr(), L.LAL_TAIL_F32, stream=st),
+            # the sum that the tail takes, directly before its step
+            lambda: L.add_rms_norm_q8(self.y.data_ptr(), self.h.data_ptr(), self.h.data_ptr(), self.norm_w.data_ptr(), 1e-6,
+                                      n, d, self.q.data_ptr(), self.s.data_ptr(), L.LAL_TAIL_F32, stream=st),
+        ]
+
+
+@pytest.mark.parametrize("streams,sampler,per_stream", [(1, L.LAL_SAMPLER_LIBRARY, False), (1, L.LAL_SAMPLER_SERVER, False),
+                                                        (3, L.LAL_SAMPLER_LIBRARY, True), (5, L.LAL_SAMPLER_LIBRARY, False),
+                                                        (1, L.LAL_SAMPLER_GPT2, False)])
+def test_chain_into_the_tail_without_waiting(monkeypatch, streams, sampler, per_stream):
+    """The tail starts while the norm before it ends, and takes the h that this
+    norm writes: the tokens are those of a run that waits after every call."""
+    if per_stream:
+        monkeypatch.setenv("LAL_TAIL_PER_STREAM", "1")
+    cfg = synth.CONFIGS["c1_gpt2"].with_(vocab=5003, n_embd=1024, hist=16)
+    b = MixedBlock(streams, 1024, 1536, 32)
+    w = (1.0 + 0.2 * np.random.default_rng(1).standard_normal(cfg.n_embd)).astype(np.float32)
+    head = synth.lm_head_f32(cfg)
+    steps = 24
+    u = torch.rand(steps, streams, generator=torch.Generator().manual_seed(2)).cuda()
+    runs = []
+    for wait in (True, False):
+        t = L.DecodeTail(cfg.vocab, cfg.n_embd, max_top_k=cfg.top_k, history_cap=cfg.hist, max_streams=streams, sampler=sampler)
+        t.load_lm_head_f32(head)
+        t.set_sampling([cfg.temperature] * streams, [cfg.top_k] * streams, [cfg.rep_penalty] * streams)
+        for k in range(streams):
+            t.set_history(k, synth.history(cfg, k))
+        if sampler != L.LAL_SAMPLER_GPT2:
+            t.set_final_norm(w, 1e-6)
+        tok = torch.empty(steps, streams, dtype=torch.int32, device="cuda")
+        b.reset()
+        torch.cuda.synchronize()
+        calls = b.calls(t.stream())
+        for step in range(steps):
+            for call in calls + [lambda: t.step_device(b.h.data_ptr(), streams, u[step].data_ptr(), tok[step].data_ptr())]:
+                call()
+                if wait:
+                    t.sync()
+        t.sync()
+        torch.cuda.synchronize()
+        runs.append((tok.cpu(), b.h.clone(), b.y.clone()))
+        t.close()
+    for one, two in zip(*runs):
+        assert torch.equal(one, two)
+    assert len(torch.unique(runs[0][0])) > 1
