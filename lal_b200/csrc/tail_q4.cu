@@ -330,10 +330,12 @@ struct MatvecParams {
  * streams and minima 13 us, 0.50), the smallest by latency (3584x3584 3.7 us).  A
  * block's word t of row g, shifted and masked, is that lane's part of the A
  * operand for columns 4t.. and 16 + 4t..: q - 8 in the upper half of a byte is
- * 16 (q - 8) as int8, so the dots come out 16 times too large and the scales
- * carry 1/16.  The dots of a group are exact int32 (below 2^24), and are
- * scaled and added in fp32.  With a minimum, w = s (q - 8) + (8 s + m): a
- * second product with rows of 16 gives 16 times the sums of the vectors. */
+ * 16 (q - 8) as int8, so the dots come out 16 times too large, which the results
+ * take back.  The dots of a group are exact int32 (below 2^24), and are scaled
+ * and added in fp32.  With a minimum, w = s q + m: A holds q itself, and a second
+ * product with rows of ones gives the sums of the vectors.  (s (q - 8) and 8 s + m
+ * would cancel where q is small, and leave 8 s of rounding: 3% of the result for
+ * groups of one large weight and many small ones.) */
 constexpr int kStageBlocks = 8;               /* 256 columns */
 /* 16 bytes to shared memory, the last 16 - n of them zeros */
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int n) {
@@ -358,6 +360,16 @@ __device__ __forceinline__ void mma_s8_zero(int (&c)[4], const uint32_t (&a)[4],
         : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
 }
+
+/* Four weights of a word, of columns j .. j + 3 or of those 16 further, as int8:
+ * 16 (q - 8), or with minima q itself.  kUnit takes the 16 out of the results. */
+template <bool kMin> __device__ __forceinline__ uint32_t low_weights(uint32_t w) {
+    return kMin ? w & 0x0f0f0f0fu : ((w << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+}
+template <bool kMin> __device__ __forceinline__ uint32_t high_weights(uint32_t w) {
+    return kMin ? (w >> 4) & 0x0f0f0f0fu : (w & 0xf0f0f0f0u) ^ 0x80808080u;
+}
+template <bool kMin> constexpr float kUnit = kMin ? 1.0f : 0.0625f;
 
 /* 16 columns c0 .. of kCount vectors, `step` bytes apart and aligned to 16 bytes,
  * of which n exist (of vector j to dst(j)); zeros behind their end. */
@@ -384,7 +396,7 @@ __device__ __forceinline__ void store_y(const MatvecParams &p, int b, int row, f
 /* A warp's results from mma accumulators: 16 kMT rows from row0 (`rows` of them
  * exist) by 8 kNT streams from b0 (nx exist).  Written out once for each type,
  * with addresses moved on: code that runs once a tile is fetched for it alone. */
-template <typename T, int kMT, int kNT>
+template <typename T, bool kMin, int kMT, int kNT>
 __device__ __forceinline__ void store_tile_as(const MatvecParams &p, int b0, int nx, int row0, int rows,
                                               const float (&acc)[kMT][kNT][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -399,16 +411,16 @@ __device__ __forceinline__ void store_tile_as(const MatvecParams &p, int b0, int
 #pragma unroll
             for (int r = 0; r < 2 * kMT; ++r)
                 if (g + 8 * r < rows)
-                    y[c * p.y_stride + 8 * r] = from_f32<T>(__fmul_rn(s, __fmul_rn(0.0625f, acc[r >> 1][n][2 * (r & 1) + c])));
+                    y[c * p.y_stride + 8 * r] = from_f32<T>(__fmul_rn(s, __fmul_rn(kUnit<kMin>, acc[r >> 1][n][2 * (r & 1) + c])));
         }
     }
 }
-template <int kMT, int kNT>
+template <bool kMin, int kMT, int kNT>
 __device__ __forceinline__ void store_tile(const MatvecParams &p, int b0, int nx, int row0, int rows,
                                            const float (&acc)[kMT][kNT][4]) {
-    if (p.dtype == LAL_TAIL_F32) store_tile_as<float>(p, b0, nx, row0, rows, acc);
-    else if (p.dtype == LAL_TAIL_BF16) store_tile_as<__nv_bfloat16>(p, b0, nx, row0, rows, acc);
-    else store_tile_as<__half>(p, b0, nx, row0, rows, acc);
+    if (p.dtype == LAL_TAIL_F32) store_tile_as<float, kMin>(p, b0, nx, row0, rows, acc);
+    else if (p.dtype == LAL_TAIL_BF16) store_tile_as<__nv_bfloat16, kMin>(p, b0, nx, row0, rows, acc);
+    else store_tile_as<__half, kMin>(p, b0, nx, row0, rows, acc);
 }
 
 /* kCount words from an even offset on */
@@ -622,7 +634,7 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
                     const int block = 2 * pair + k;
                     const bool begin = block % kPer == 0;
                     if (kMin) {
-                        const uint32_t ones[4] = {0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u};
+                        const uint32_t ones[4] = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
 #pragma unroll
                         for (int n = 0; n < kNT; ++n) {
                             if (begin) mma_s8_zero(cx[n], ones, x[n][2 * k], x[n][2 * k + 1]);
@@ -632,8 +644,7 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
 #pragma unroll
                     for (int m = 0; m < kMT; ++m) {
                         const uint32_t w0 = w[m][2 * k], w1 = w[m][2 * k + 1];
-                        const uint32_t a[4] = {((w0 << 4) & 0xf0f0f0f0u) ^ 0x80808080u, ((w1 << 4) & 0xf0f0f0f0u) ^ 0x80808080u,
-                                               (w0 & 0xf0f0f0f0u) ^ 0x80808080u, (w1 & 0xf0f0f0f0u) ^ 0x80808080u};
+                        const uint32_t a[4] = {low_weights<kMin>(w0), low_weights<kMin>(w1), high_weights<kMin>(w0), high_weights<kMin>(w1)};
 #pragma unroll
                         for (int n = 0; n < kNT; ++n) {
                             if (begin) mma_s8_zero(c[m][n], a, x[n][2 * k], x[n][2 * k + 1]);
@@ -644,7 +655,7 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const float s = __half2float(scale[m][h].one[gr]);
-                            const float l = kMin ? fmaf(8.0f, s, __half2float(low[m][h].one[gr])) : 0.0f;
+                            const float l = kMin ? __half2float(low[m][h].one[gr]) : 0.0f;
 #pragma unroll
                             for (int n = 0; n < kNT; ++n)
 #pragma unroll
@@ -663,7 +674,7 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
         after_previous();
     }
     if (warps_k == 1) {
-        if (live) store_tile(p, b0, nx, row0, min(height, p.rows - row0), acc);
+        if (live) store_tile<kMin>(p, b0, nx, row0, min(height, p.rows - row0), acc);
         return;
     }
     /* the warps of a row tile, in order; their sums take the rings' place */
@@ -684,7 +695,7 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
         if (r >= height || row >= p.rows) continue;
         float sum = 0.0f;
         for (int w = 0; w < warps_k; ++w) sum += part[tile * warps_k + w][b * kRows + r];
-        store_y(p, b0 + b, row, 0.0625f * sum);
+        store_y(p, b0 + b, row, kUnit<kMin> * sum);
     }
 }
 
@@ -717,7 +728,7 @@ cudaError_t launch_mma(const MatvecParams &p, int x_base, int num_sms, cudaStrea
  * A CTA takes tiles of 128 rows by up to 64 streams.  The weights are the A
  * operand and lie in tensor memory: a thread of the eight unpacking warps has a
  * row, reads its 16-byte blocks from a ring of its warp's own (cp.async) and
- * stores 16 (q - 8) as int8, eight columns of tensor memory a block.  The
+ * stores 16 (q - 8), or with minima q, as int8, eight columns of tensor memory a block.  The
  * vectors are the B operand, in shared memory with the 128-byte swizzle.  One
  * thread issues the products, two groups of columns at a time into two of kTcD
  * accumulators; sixteen warps read finished ones (int32, exact), scale them
@@ -798,12 +809,12 @@ __device__ __forceinline__ void tc_load16(uint32_t at, int (&r)[16]) {
 }
 
 /* A thread's results, n of kCount streams from b0, of a row. */
-template <typename T, int kCount>
+template <typename T, bool kMin, int kCount>
 __device__ __forceinline__ void store_row(const MatvecParams &p, int b0, int n, int row, const float (&acc)[kCount]) {
     T *y = (T *)p.y + (size_t)b0 * p.y_stride + row;
 #pragma unroll
     for (int j = 0; j < kCount; ++j, y += p.y_stride)
-        if (j < n) *y = from_f32<T>(__fmul_rn(p.sx[b0 + j], __fmul_rn(0.0625f, acc[j])));
+        if (j < n) *y = from_f32<T>(__fmul_rn(p.sx[b0 + j], __fmul_rn(kUnit<kMin>, acc[j])));
 }
 
 /* The stages of a CTA in order: every tile's range of K. */
@@ -929,8 +940,8 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                 uint32_t o[8];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    o[j] = ((w[j] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
-                    o[4 + j] = (w[j] & 0xf0f0f0f0u) ^ 0x80808080u;
+                    o[j] = low_weights<kMin>(w[j]);
+                    o[4 + j] = high_weights<kMin>(w[j]);
                 }
                 tc_store8(to + buf * 64 + i * 8, o);
             }
@@ -985,7 +996,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
 #pragma unroll
                     for (int j = 0; j < kMine; ++j) acc[j] = fmaf(s, (float)c[j], acc[j]);
                     if (kMin) {
-                        const float m = fmaf(8.0f, s, __half2float(__ushort_as_half(low.one[gr])));
+                        const float m = __half2float(__ushort_as_half(low.one[gr]));
                         const float4 *sum = (const float4 *)(xsums + (xs * kGroups + gr) * kN + part * kMine);
 #pragma unroll
                         for (int j = 0; j < kMine; j += 4) {
@@ -1006,9 +1017,9 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             if (splits == 1 && at.st == st1 - 1) {
                 const int row = at.tile * 128 + quad * 32 + lane;
                 if (row < p.rows) {
-                    if (p.dtype == LAL_TAIL_F32) store_row<float>(p, b0 + part * kMine, nx - part * kMine, row, acc);
-                    else if (p.dtype == LAL_TAIL_BF16) store_row<__nv_bfloat16>(p, b0 + part * kMine, nx - part * kMine, row, acc);
-                    else store_row<__half>(p, b0 + part * kMine, nx - part * kMine, row, acc);
+                    if (p.dtype == LAL_TAIL_F32) store_row<float, kMin>(p, b0 + part * kMine, nx - part * kMine, row, acc);
+                    else if (p.dtype == LAL_TAIL_BF16) store_row<__nv_bfloat16, kMin>(p, b0 + part * kMine, nx - part * kMine, row, acc);
+                    else store_row<__half, kMin>(p, b0 + part * kMine, nx - part * kMine, row, acc);
                 }
             }
         }
@@ -1103,7 +1114,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             cp_async_wait<kTcXDepth - 2>();
             __syncwarp();
             if (kMin) {
-                /* 16 times the sum of each group of this warp's rows */
+                /* the sum of each group of this warp's rows */
                 const uint8_t *st = xring + xs * kTcXStage;
                 for (int i = lane; i < kN / kTcLoad * kGroups; i += 32) {
                     const int gr = i % kGroups, pair = i / kGroups;
@@ -1114,8 +1125,8 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                     for (int j = 0; j < kPer * 2; ++j) {
                         const int c = gr * kPer * 2 + j;
                         const uint4 v = *(const uint4 *)(st + (c >> 3) * kN * 128 + n * 128 + (((c & 7) ^ (n & 7)) << 4));
-                        sum = __dp4a((int)v.x, 0x10101010, __dp4a((int)v.y, 0x10101010, sum));
-                        sum = __dp4a((int)v.z, 0x10101010, __dp4a((int)v.w, 0x10101010, sum));
+                        sum = __dp4a((int)v.x, 0x01010101, __dp4a((int)v.y, 0x01010101, sum));
+                        sum = __dp4a((int)v.z, 0x01010101, __dp4a((int)v.w, 0x01010101, sum));
                     }
                     xsums[(xs * kGroups + gr) * kN + n] = (float)sum;
                 }
@@ -1162,7 +1173,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             if (n >= nx || row >= p.rows) continue;
             float sum = 0.0f;
             for (int s = 0; s < splits; ++s) sum += parts[((size_t)s * mine + (i >> 7)) * 128 + (i & 127)];
-            store_y(p, b0 + n, row, 0.0625f * sum);
+            store_y(p, b0 + n, row, kUnit<kMin> * sum);
         }
     }
     tc_fence_before();
@@ -1321,10 +1332,10 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
                         ldmatrix4(w, (a_at + at + m * 2048) ^ ((u * (kUnit / 2) + q) << 5));
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            a[m][2 * q + k][0] = ((w[2 * k] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
-                            a[m][2 * q + k][1] = ((w[2 * k + 1] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
-                            a[m][2 * q + k][2] = (w[2 * k] & 0xf0f0f0f0u) ^ 0x80808080u;
-                            a[m][2 * q + k][3] = (w[2 * k + 1] & 0xf0f0f0f0u) ^ 0x80808080u;
+                            a[m][2 * q + k][0] = low_weights<kMin>(w[2 * k]);
+                            a[m][2 * q + k][1] = low_weights<kMin>(w[2 * k + 1]);
+                            a[m][2 * q + k][2] = high_weights<kMin>(w[2 * k]);
+                            a[m][2 * q + k][3] = high_weights<kMin>(w[2 * k + 1]);
                         }
                     }
                 float s[kMT][2][kUnitGroups], l[kMT][2][kUnitGroups];
@@ -1344,8 +1355,7 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
 #pragma unroll
                         for (int k = 0; k < kUnitGroups; ++k) {
                             s[m][r][k] = __half2float(__ushort_as_half((unsigned short)(v >> (16 * k))));
-                            if (kMin)
-                                l[m][r][k] = fmaf(8.0f, s[m][r][k], __half2float(__ushort_as_half((unsigned short)(w >> (16 * k)))));
+                            if (kMin) l[m][r][k] = __half2float(__ushort_as_half((unsigned short)(w >> (16 * k))));
                         }
                     }
                 /* kB eights of vectors at once: as many independent products again */
@@ -1370,7 +1380,7 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
                             for (int n = 0; n < kB; ++n) {
                                 const uint32_t x0 = x[n][i / 2][2 * (i % 2)], x1 = x[n][i / 2][2 * (i % 2) + 1];
                                 if (kMin) {
-                                    const uint32_t ones[4] = {0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u};
+                                    const uint32_t ones[4] = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
                                     if (j == 0) mma_s8_zero(cx[n], ones, x0, x1);
                                     else mma_s8(cx[n], ones, x0, x1);
                                 }
@@ -1398,7 +1408,7 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
         if (++slot == kWideDepth) slot = 0;
         if (++st < stages) continue;
         st = 0;
-        store_tile(p, b0, nx, row0, min(h.height, end - row0), acc);
+        store_tile<kMin>(p, b0, nx, row0, min(h.height, end - row0), acc);
         row0 += tile_rows;
     }
     cp_async_wait<0>();

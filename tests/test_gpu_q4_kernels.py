@@ -172,3 +172,21 @@ def test_aligned_values_of_every_kind(streams, rows, cols, group, minimum):
     ok = ~np.isnan(want)
     with np.errstate(invalid="ignore"):
         assert np.all((np.abs(got - want) <= bound(want, size, cols, "f32"))[ok])
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("streams,rows,cols", ONE_EACH + [(5, 300, 1000), (20, 300, 1000)])
+def test_minima_far_below_their_scales(streams, rows, cols, group):
+    """Groups of one large weight and many small ones, as an outlier makes
+    them: where q is 0 the weight is the minimum alone, and no term of the
+    scale's size enters the sum."""
+    c = Case(streams, rows, cols, group, True)
+    c.s.copy_((c.s.float() * 1e4).half())
+    c.m.copy_((c.m.float() * 1e-2).half())
+    c.q.zero_()
+    c.x[:, ::group] = 0
+    c.q[:, ::group // 2] |= 15  # the first column of each group, and x there is 0
+    c.check(c.run())
+    c.x[:, group // 2::group] = 0
+    c.q[:, :16] = 0x21  # a block of small q's among them
+    c.check(c.run())
