@@ -928,11 +928,11 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
             for (int i = 0; i < kTcHalf; ++i) v[i] = *(const uint4 *)(row + ((i ^ ((lane >> 1) & 3)) << 4));
             slot = slot + 1 == kTcWDepth ? 0 : slot + 1;
             const int buf = it % kTcA;
-            if (it >= kTcA && !tc_wait(&sh.a_empty[buf], ((it / kTcA) & 1) ^ 1, abort_flag)) {
+            const bool ok = it < kTcA || tc_wait(&sh.a_empty[buf], ((it / kTcA) & 1) ^ 1, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) { /* a warp leaves as one: what follows is for all its lanes */
                 *abort_flag = 1;
                 break;
             }
-            __syncwarp();
             tc_fence_after();
 #pragma unroll
             for (int i = 0; i < kTcHalf; ++i) {
