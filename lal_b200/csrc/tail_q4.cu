@@ -547,11 +547,8 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
                         const int n = (int)max(0LL, min(16LL, (long long)(end - from) - 16 * e));
                         cp_async16_l1(smem_u32(to + 16 * e), n > 0 ? from + 16 * e : from, n);
                     }
-                } else if (g0 + kGroups <= groups) {
+                } else { /* a row of scales is whole stages (all_aligned) */
                     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(row + g0), "n"(2 * kGroups) : "memory");
-                } else {
-#pragma unroll
-                    for (int k = 0; k < kGroups; ++k) ((unsigned short *)to)[k] = g0 + k < groups ? row[g0 + k] : 0;
                 }
             }
         };
@@ -614,7 +611,7 @@ __global__ void __launch_bounds__(kFill == kMany ? 384 : 256, kMT * kNT == 1 ? 2
             int c[kMT][kNT][4], cx[kNT][4];
 #pragma unroll
             for (int pair = 0; pair < kStageBlocks / 2; ++pair) {
-                /* blocks behind the row's end hold zeros in the vectors, and their groups scales of zero */
+                /* blocks behind the row's end hold zeros in the vectors; groups behind it (kAny) scales of zero */
                 uint32_t w[kMT][4], x[kNT][4];
 #pragma unroll
                 for (int m = 0; m < kMT; ++m) ldmatrix4(w[m], (at + a_at + m * 2048) ^ (pair << 5));
@@ -1097,12 +1094,7 @@ __global__ void __launch_bounds__(32 * kTcWarps, 1) q4_tc_kernel(const MatvecPar
                 for (int m = 0; m < (kMin ? 2 : 1); ++m) {
                     const unsigned short *src = (const unsigned short *)(m ? p.min : p.scale) + (size_t)row * groups + g0;
                     uint8_t *to = sring + ((xs * (kMin ? 2 : 1) + m) * 128 + lw * 32 + lane) * (2 * kGroups);
-                    if (g0 + kGroups <= groups) {
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(src), "n"(2 * kGroups) : "memory");
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < kGroups; ++k) ((unsigned short *)to)[k] = g0 + k < groups ? src[k] : 0;
-                    }
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(src), "n"(2 * kGroups) : "memory");
                 }
             }
             ahead.next(st0, st1, tile_step);
@@ -1281,15 +1273,7 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
                 for (int m = 0; m < (kMin ? 2 : 1); ++m) {
                     const unsigned short *src = (const unsigned short *)(m ? p.min : p.scale) + s_row + g0;
                     const uint32_t dst = w_ring + base + Stage::kA + m * Stage::kScale + lane * (2 * kGroups);
-                    if (g0 + kGroups <= groups) {
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(2 * kGroups) : "memory");
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < kGroups; ++k) {
-                            const unsigned short v = g0 + k < groups ? src[k] : 0;
-                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + 2 * k), "h"(v) : "memory");
-                        }
-                    }
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(2 * kGroups) : "memory");
                 }
             }
             --l_left;
@@ -1319,7 +1303,7 @@ __global__ void __launch_bounds__(512 / kWideMT, 1) q4_wide_kernel(const MatvecP
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
         if (row0 < end) {
-            /* blocks behind the row's end hold zeros in the vectors, and their groups scales of zero */
+            /* blocks behind the row's end hold zeros in the vectors */
             const uint32_t at = slot * Stage::kW, xt = slot * Stage::kX;
 #pragma unroll 1
             for (int u = 0; u < kUnits; ++u) {
@@ -1429,8 +1413,10 @@ cudaError_t launch_wide(const MatvecParams &p, int x_base, int num_sms, cudaStre
                         1, p, h, x_base);
 }
 
-/* Whether every vector and every row of scales begins where copies of 16 bytes
- * (scales: of a stage's) may. */
+/* Whether every vector begins at a 16-byte boundary and every row of scales at
+ * one of a stage's copy, 512 / group bytes, of which it then holds whole ones.
+ * (So columns that are no multiple of 256, but for a last stage whose groups
+ * are all begun, count as not aligned.) */
 inline bool all_aligned(const MatvecParams &p) {
     const int groups = (p.cols + p.group - 1) / p.group, copy = 2 * kStageBlocks * kQ4Block / p.group;
     return (uintptr_t)p.x % 16 == 0 && (p.streams == 1 || p.x_stride % 16 == 0) &&
