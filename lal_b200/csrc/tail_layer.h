@@ -14,6 +14,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 
 namespace lal {
 
@@ -33,17 +34,26 @@ inline int dtype_size(int dtype) {
     return dtype == LAL_TAIL_F32 ? 4 : dtype == LAL_TAIL_BF16 || dtype == LAL_TAIL_F16 ? 2 : 0;
 }
 
-/* The bytes that `rows` rows of `n` elements, `stride` elements apart, span. */
+/* The bytes that `rows` rows of `n` elements, `stride` elements apart, span;
+ * `fits` where they end within the address space. */
 struct Span {
     uintptr_t lo = 0, hi = 0;
+    bool fits = true;
     Span() {}
     Span(const void *p, long long rows, long long n, long long stride, int size) {
         if (p == nullptr || rows < 1) return;
+        const unsigned __int128 end = (uintptr_t)p + ((unsigned __int128)(rows - 1) * (unsigned long long)stride + n) * size;
+        fits = end <= UINTPTR_MAX;
         lo = (uintptr_t)p;
-        hi = lo + (uintptr_t)((rows - 1) * stride + n) * size;
+        hi = fits ? (uintptr_t)end : UINTPTR_MAX;
     }
     bool meets(const Span &o) const { return lo < o.hi && o.lo < hi; }
 };
+inline bool all_fit(std::initializer_list<Span> spans) {
+    for (const Span &s : spans)
+        if (!s.fits) return false;
+    return true;
+}
 
 /* The device whose memory p is; host memory is refused here, before a kernel
  * could fault on it. */

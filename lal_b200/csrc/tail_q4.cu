@@ -1523,7 +1523,9 @@ int convert_q4(const char *op, const lal_tail_q4 *w, void *d_w, int64_t w_stride
     if ((uintptr_t)d_w % size != 0)
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: a pointer is not aligned to its type", op);
     const WeightSpans spans(w);
-    if (spans.meets(Span(d_w, w->rows, w->cols, w_stride, size)) || spans.meet_each_other())
+    const Span values(d_w, w->rows, w->cols, w_stride, size);
+    if (!values.fits) return layer_fail(LAL_TAIL_ERR_ARG, "%s: a stride beyond the address space", op);
+    if (spans.meets(values) || spans.meet_each_other())
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: buffers overlap", op);
     if (q4_ctas(w->rows, w->cols) > 0x7fffffffLL)
         return layer_fail(LAL_TAIL_ERR_UNSUPPORTED, "%s: weights of %d x %d", op, w->rows, w->cols);
@@ -1569,8 +1571,9 @@ int lal_tail_q4_matvec(const lal_tail_q4 *w, const int8_t *d_xq, int64_t xq_stri
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: a stride below the weights' %d x %d", op, w->rows, w->cols);
     if ((uintptr_t)d_y % size != 0 || (uintptr_t)d_scale_x % 4 != 0)
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: a pointer is not aligned to its type", op);
-    const Span y(d_y, n_streams, w->rows, y_stride, size);
-    if (y.meets(Span(d_xq, n_streams, w->cols, xq_stride, 1)) ||
+    const Span y(d_y, n_streams, w->rows, y_stride, size), x(d_xq, n_streams, w->cols, xq_stride, 1);
+    if (!all_fit({y, x})) return layer_fail(LAL_TAIL_ERR_ARG, "%s: a stride beyond the address space", op);
+    if (y.meets(x) ||
         y.meets(Span(d_scale_x, 1, n_streams, n_streams, 4)) || WeightSpans(w).meets(y))
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: an output overlaps another buffer", op);
     static const char *const names[] = {"d_xq", "d_scale_x", "d_y", "d_q", "d_scale", "d_min"};

@@ -546,6 +546,7 @@ int lal_tail_add_rms_norm_q8(const void *d_x, int64_t x_stride, const void *d_re
     const Span x(d_x, rows, n_embd, x_stride, size), r(d_residual, rows, n_embd, residual_stride, size),
         h(d_h, rows, n_embd, h_stride, size), w(d_norm_w, 1, n_embd, n_embd, 4),
         q(d_q, rows, n_embd, q_stride, 1), s(d_scale, 1, rows, rows, 4);
+    if (!all_fit({x, r, h, q})) return layer_fail(LAL_TAIL_ERR_ARG, "%s: a stride beyond the address space", op);
     const bool h_on_x = d_h == d_x && h_stride == x_stride;
     const bool h_on_r = d_residual && d_h == d_residual && h_stride == residual_stride;
     if ((!h_on_x && h.meets(x)) || (!h_on_r && h.meets(r)) || h.meets(w) || h.meets(q) || h.meets(s) ||
@@ -579,6 +580,7 @@ int lal_tail_swiglu_q8(const void *d_gate, int64_t gate_stride, const void *d_up
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: a pointer is not aligned to its type", op);
     const Span g(d_gate, rows, n, gate_stride, size), u(d_up, rows, n, up_stride, size),
         q(d_q, rows, n, q_stride, 1), s(d_scale, 1, rows, rows, 4);
+    if (!all_fit({g, u, q})) return layer_fail(LAL_TAIL_ERR_ARG, "%s: a stride beyond the address space", op);
     if (q.meets(g) || q.meets(u) || q.meets(s) || s.meets(g) || s.meets(u))
         return layer_fail(LAL_TAIL_ERR_ARG, "%s: an output overlaps another buffer", op);
     static const char *const names[] = {"d_gate", "d_up", "d_q", "d_scale"};
