@@ -381,7 +381,8 @@ int lal_tail_debug_expf(const float *x, float *y, int n);
  * captured.  Zero rows or streams: nothing is done; rows and columns go up to
  * 2^30 (rows of the 8-bit operators up to 2^31 - 1).  Only the rows and columns
  * named are written, and no output may overlap another buffer of the call,
- * except where a call says so.  A row's results do not depend on what the
+ * except where a call says so (columns of one buffer, the same number of bytes
+ * from row to row, do not overlap).  A row's results do not depend on what the
  * other rows or streams of a call hold, and are the same in every run. */
 #define LAL_TAIL_F32  0
 #define LAL_TAIL_BF16 1

@@ -35,9 +35,10 @@ inline int dtype_size(int dtype) {
 }
 
 /* The bytes that `rows` rows of `n` elements, `stride` elements apart, span;
- * `fits` where they end within the address space. */
+ * `fits` where they end within the address space.  Rows that lie between
+ * another buffer's, `step` bytes apart as those are, do not meet them. */
 struct Span {
-    uintptr_t lo = 0, hi = 0;
+    uintptr_t lo = 0, hi = 0, width = 0, step = 0; /* step 0: one row */
     bool fits = true;
     Span() {}
     Span(const void *p, long long rows, long long n, long long stride, int size) {
@@ -46,8 +47,16 @@ struct Span {
         fits = end <= UINTPTR_MAX;
         lo = (uintptr_t)p;
         hi = fits ? (uintptr_t)end : UINTPTR_MAX;
+        width = (uintptr_t)n * size;
+        step = fits && rows > 1 ? (uintptr_t)stride * size : 0;
     }
-    bool meets(const Span &o) const { return lo < o.hi && o.lo < hi; }
+    bool meets(const Span &o) const {
+        if (!(lo < o.hi && o.lo < hi)) return false;
+        const uintptr_t s = step != 0 ? step : o.step;
+        if (s == 0 || (o.step != 0 && o.step != s)) return true;
+        const uintptr_t at = o.lo >= lo ? (o.lo - lo) % s : (s - (lo - o.lo) % s) % s; /* of o's rows behind these */
+        return at < width || o.width > s - at;
+    }
 };
 inline bool all_fit(std::initializer_list<Span> spans) {
     for (const Span &s : spans)

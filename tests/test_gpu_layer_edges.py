@@ -5,12 +5,13 @@ import numpy as np
 import pytest
 
 import lal_b200 as L
+import layer_ref as ref
 from lal_b200 import synth
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_layer_ops import Weights, check_rows, run_swiglu, stream  # noqa: E402
+from test_gpu_layer_ops import Weights, check_rows, f64, run_swiglu, stream  # noqa: E402
 
 
 # ---- SwiGLU at gates that 32-bit intermediates do not hold --------------------------------
@@ -126,3 +127,29 @@ def test_chain_into_the_tail_without_waiting(monkeypatch, streams, sampler, per_
     for one, two in zip(*runs):
         assert torch.equal(one, two)
     assert len(torch.unique(runs[0][0])) > 1
+
+
+# ---- columns of one buffer ----------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,n", [(3, 64), (5, 1001), (301, 256)])
+def test_operators_within_one_buffer(rows, n):
+    """Rows of one record each: x, residual, h and q of the norm, gate, up and
+    q of the SwiGLU, side by side."""
+    rng = np.random.default_rng(n)
+    x, r = rng.standard_normal((2, rows, n))
+    w = (1 + 0.1 * rng.standard_normal(n)).astype(np.float32)
+    step = 4 * n + 4  # in fp32: x, residual, h, q (in n / 4 of them) and a gap
+    whole = torch.full((rows, step), 77.0, device="cuda")
+    whole[:, :n], whole[:, n:2 * n] = torch.as_tensor(x), torch.as_tensor(r)
+    at, dw, s = whole.data_ptr(), torch.as_tensor(w).cuda(), torch.empty(rows, device="cuda")
+    h = whole[:, :n] + whole[:, n:2 * n]
+    L.add_rms_norm_q8(at, at + 4 * n, at + 8 * n, dw.data_ptr(), 1e-6, rows, n, at + 12 * n, s.data_ptr(), x_stride=step,
+                      residual_stride=step, h_stride=step, q_stride=4 * step, stream=stream())
+    torch.cuda.synchronize()
+    q = whole.view(torch.int8)[:, 12 * n:13 * n]
+    assert torch.equal(whole[:, 2 * n:3 * n], h)
+    check_rows(q, s, *ref.norm_q8(f64(h), w, 1e-6))
+    L.swiglu_q8(at, at + 4 * n, rows, n, at + 8 * n, s.data_ptr(), gate_stride=step, up_stride=step, q_stride=4 * step, stream=stream())
+    torch.cuda.synchronize()
+    check_rows(whole.view(torch.int8)[:, 8 * n:9 * n], s, *ref.swiglu_q8(f64(whole[:, :n]), f64(whole[:, n:2 * n])))
+    assert bool((whole[:, -3:] == 77.0).all())
