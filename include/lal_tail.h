@@ -434,7 +434,7 @@ typedef struct {
  * scale = max|w| / 7 of the group, q = rint(w / scale) + 8.  With one: min =
  * the group's smallest value, scale = (its largest - min) / 15, q = rint((w -
  * min) / scale).  Scales are rounded up to f16 and minima down, so no weight
- * is clamped; q is taken with the rounded ones, as in 64 bits (ties to
+ * is clamped; q is the exact quotient with the rounded ones, rounded (ties to
  * even).  A group with a value that is not finite, or too large for an f16
  * scale, gets scale (and minimum) NaN. */
 int lal_tail_quantize_q4(const lal_tail_q4 *w, const void *d_w, int64_t w_stride, int dtype,
@@ -444,8 +444,10 @@ int lal_tail_dequantize_q4(const lal_tail_q4 *w, void *d_w, int64_t w_stride, in
 /* y[b, r] = d_scale_x[b] * sum over columns c of xq[b, c] * weight[r, c], for
  * n_streams (at most LAL_TAIL_Q4_MAX_STREAMS) 8-bit vectors; y is [n_streams,
  * w->rows] of `dtype`.  The dots of 32 columns are exact integers, their
- * scaled sum is held in fp32.  xq may hold -128.  Vectors and rows of scales at
- * 16-byte boundaries are read fastest.  (Beside
+ * scaled sum is held in fp32.  xq may hold -128.  The fast forms want every
+ * vector at a 16-byte boundary, and LAL_TAIL_Q4_GROUPS(cols, group) a multiple of
+ * 256 / group with d_scale and d_min aligned to 512 / group bytes: cols a multiple
+ * of 256, or up to group - 1 fewer.  Others take 16 streams at a time.  (Beside
  * lal_lm_head_int8_range, runtime/lal_q8_kernel.h:463; the 4-bit products of
  * the server's layers.) */
 int lal_tail_q4_matvec(const lal_tail_q4 *w, const int8_t *d_xq, int64_t xq_stride,

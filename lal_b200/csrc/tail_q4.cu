@@ -101,9 +101,9 @@ template <typename T> union Four {
 };
 
 /* Both directions: four lanes a block, a warp takes kRun runs of 256 columns of
- * a row, all their loads at once.  Bounded by HBM: 18944x3584 fp32 to 4 bits 54
- * us (0.86 of the measured rate), back 47.5 (0.98); bf16 61 us, bounded by
- * instructions, and 32.  Of fp32, lane u of a block has columns 4u ..
+ * a row, all their loads at once.  Bounded by HBM: 18944x3584 fp32 to 4 bits 53
+ * us (0.88 of the measured rate; with minima and groups of 32 69), back 47.3
+ * (0.99); bf16 60 us (108), bounded by instructions, and 32.  Of fp32, lane u of a block has columns 4u ..
  * 4u + 3 and 16 + 4u .., which are the word u; of 16-bit numbers eight columns
  * in a row, 16 bytes, and half a word's worth goes over to another lane. */
 constexpr int kRun = 4;
@@ -319,15 +319,15 @@ struct MatvecParams {
     int dtype;
 };
 
-/* ---- up to sixteen streams: mma.sync m16n8k32 on int8 ----
+/* ---- up to sixteen streams at a time: mma.sync m16n8k32 on int8 ----
  *
  * A warp takes 16 kMT rows and every warps_k-th stage of 256 columns; the rows'
  * 4-bit words, their scales and the vectors go through a ring of shared memory
  * of its own (cp.async, no barrier of the CTA until the warps' sums are joined).
- * Large weights are read at 0.74 to 0.86 of the measured HBM rate (152064x3584
- * with one stream 56 us, with sixteen 58); few rows are bounded by a warp's
+ * Large weights are read at 0.76 to 0.86 of the measured HBM rate (152064x3584
+ * with one stream 55 us, with sixteen 58); few rows are bounded by a warp's
  * instructions a stage, about 22 a block and 16 rows (3584x18944 with eight
- * streams and minima 13 us, 0.50), the smallest by latency (3584x3584 3.7 us).  A
+ * streams and minima 11.8 us, 0.55), the smallest by latency (3584x3584 3.6 us).  A
  * block's word t of row g, shifted and masked, is that lane's part of the A
  * operand for columns 4t.. and 16 + 4t..: q - 8 in the upper half of a byte is
  * 16 (q - 8) as int8, so the dots come out 16 times too large, which the results
@@ -446,9 +446,10 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
  * 16-byte boundaries (scales: of a stage's size) and lie as ldmatrix wants
  * them.  kAny: the aligned 16-byte pieces around them are copied as they are
  * (each holds a byte of its row, so none lies outside memory), and their
- * offsets are taken at the reading, so these copies are asynchronous too.  kMany (aligned, 32 rows a warp, tiles for several waves): more warps
- * with shorter rings; 58 us against 68 for 152064x3584 g128 and sixteen streams,
- * but 30 against 17 for 37888x3584, one wave. */
+ * offsets are taken at the reading, so these copies are asynchronous too.  kMany
+ * (aligned, 32 rows a warp, tiles for several waves): more warps with shorter
+ * rings; 58 us against 66 for 152064x3584 g128 and sixteen streams, but 19.3
+ * against 14.8 for 37888x3584, one wave. */
 enum MmaFill { kAligned, kMany, kAny };
 
 /* What a warp's ring holds a stage: weights of 16 kMT rows, their scales (and
@@ -1193,7 +1194,7 @@ cudaError_t launch_tc(const MatvecParams &p, int x_base, int chunks, int num_sms
 
 /* ---- 17 to 32 streams, many rows: the same products, the vectors shared by a CTA ----
  *
- * 37888x3584 g128 with 32 streams 22.3 us, 0.50 of HBM's rate; bounded by the
+ * 37888x3584 g128 with 32 streams 21.7 us, 0.53 of HBM's rate; bounded by the
  * ldmatrix traffic of the vectors and the latency of eight warps an SM.
  *
  * A CTA of eight warps takes a range of rows, 32 a warp and tile, by up to 8
@@ -1426,17 +1427,18 @@ inline bool all_aligned(const MatvecParams &p) {
 /* Which kernel for the last (at most 64) streams, from x_base on.  Measured on a
  * B200, back to back, us:
  *   streams  weights            mma    shared vectors  tcgen05
- *   16       152064x3584 g128   58     97              115
- *   16       37888x3584  g32    25.2   29.2            53.0
- *   32       37888x3584  g128   29.0   22.3            29.7
- *   32       37888x3584  g32    46.0   29.8            53.0
- *   32       3584x3584   g32    10.5   26.8            13.9
- *   64       37888x3584  g128   56.7                   30.4
- *   64       37888x3584  g32    85.8                   53.5
- *   64       3584x3584   g32    19.5                   14.4
- * so mma up to 16 streams, shared vectors up to 32 where every SM has 128
- * rows, tcgen05 beyond (and for whole 64s).  What is not aligned takes mma, 16
- * streams at a time. */
+ *   16       152064x3584 g128   58     92              114
+ *   16       37888x3584  g32    23.9   27.3            52.7
+ *   32       37888x3584  g128   27.7   21.7            29.8
+ *   32       37888x3584  g32    42.8   28.8            52.9
+ *   32       3584x3584   g32    10.5   25.4            14.1
+ *   64       37888x3584  g128   54.0                   30.6
+ *   64       37888x3584  g32    79.1                   53.4
+ *   64       3584x3584   g32    19.3                   14.5
+ * so mma up to 16 streams; of 17 to 32, shared vectors where every SM has 128
+ * rows and mma, 16 at a time, where it has fewer; tcgen05 beyond (and for whole
+ * 64s).  What is not aligned takes mma, 16 streams at a time: 37888x3584 g128
+ * 31.7 us with 16 (aligned 14.8), 62 with 32 and 124 with 64. */
 template <int kGroup, bool kMin>
 cudaError_t launch_streams(const MatvecParams &p, int x_base, int num_sms, cudaStream_t st) {
     const int n = p.streams - x_base;
@@ -1453,8 +1455,8 @@ cudaError_t launch_streams(const MatvecParams &p, int x_base, int num_sms, cudaS
         return waves ? launch_mma<2, 2, kGroup, kMin, kMany>(p, x_base, num_sms, st)
                      : launch_mma<2, 2, kGroup, kMin, kAligned>(p, x_base, num_sms, st);
     /* 32 rows a warp share its part of the vectors: fewer instructions, but half the warps.  Eight
-     * streams, us: 13.9 against 18.4 for 37888x3584 g32, 13.0 against 17.1 for 3584x18944 with minima,
-     * 3.4 against 2.9 for 5000x1024 */
+     * streams, us: 14.0 against 18.4 for 37888x3584 g32, 11.8 against 15.6 for 3584x18944 with minima,
+     * 3.3 against 2.9 for 5000x1024 */
     if (waves) return launch_mma<2, 1, kGroup, kMin, kMany>(p, x_base, num_sms, st);
     if (large) return launch_mma<2, 1, kGroup, kMin, kAligned>(p, x_base, num_sms, st);
     return launch_mma<1, 1, kGroup, kMin, kAligned>(p, x_base, num_sms, st);

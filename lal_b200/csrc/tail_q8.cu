@@ -401,9 +401,11 @@ template <typename Row> struct RowQuant {
 
 /* A row a CTA, or (kCluster) a cluster: 8 kC elements a thread, which stay in
  * registers between the statistics and the quantizer.  Norm of 4096x3584 bf16
- * with its residual 26 us (0.60 of the measured HBM rate), SwiGLU of 512x18944
- * bf16 24.5 us (0.30): bounded by latency between the two barriers and by
- * instructions, 27 and 39 an element.  One row: 2.4 and 2.9 us. */
+ * with its residual 26.4 us (0.60 of the measured HBM rate; fp32 35.5, 0.82),
+ * SwiGLU of 512x18944 bf16 24.6 us (0.30; fp32 28.6, 0.47): bounded by latency, a
+ * row's loads, barriers and stores one after the other with nothing of the next
+ * row in flight (the instructions, 27 and 39 an element, are 10 us of issue at
+ * most).  One row of 3584 and of 18944: 2.4 and 3.0 us. */
 template <typename Row, int kC, int kMaxThreads, int kMinCtas, bool kCluster>
 __global__ void __launch_bounds__(kMaxThreads, kMinCtas) row_q8_kernel(const RowParams p) {
     after_previous();
@@ -492,10 +494,10 @@ constexpr int kFewN = 8192, kFewPart = 2048;
 template <typename Row> cudaError_t launch_row(RowParams p, int rows, int num_sms, cudaStream_t st) {
     p.inv_n = 1.0f / (float)p.n;
     /* Few rows: a thread takes 8 elements, and a long row is spread over as
-     * many SMs as a cluster has (SwiGLU of one row of 18944: 9.2 us in one CTA,
-     * 5.0 over a cluster).  Many: 16 elements, and no more CTAs a row than its
-     * registers need; SwiGLU's in smaller CTAs (512 rows: 25 us against 35 with
-     * CTAs of 512 threads), the norm's in larger ones (26.4 against 27.5). */
+     * many SMs as a cluster has (SwiGLU of one row of 18944: 8.7 us in one CTA,
+     * 3.0 over a cluster).  Many: 16 elements, and no more CTAs a row than its
+     * registers need; SwiGLU's in smaller CTAs (512 rows: 24.6 us against 31.4 with
+     * CTAs of 512 threads), the norm's in larger ones (26.4 against 27.4). */
     if (rows < 2 * num_sms) {
         if (p.n <= kFewN) return launch_parts<Row, 1, 1024, 1>(p, rows, 1, st);
         if (p.n <= kMaxParts * 8192) return launch_parts<Row, 1, 1024, 1>(p, rows, std::min(kMaxParts, (p.n + kFewPart - 1) / kFewPart), st);
@@ -507,7 +509,10 @@ template <typename Row> cudaError_t launch_row(RowParams p, int rows, int num_sm
 }
 
 /* kWide where every row of every buffer begins at a 16-byte boundary (q: 8)
- * and ends at a whole eight: no test of alignment or of the end an element. */
+ * and ends at a whole eight: no test of alignment or of the end an element.
+ * Against the other form on the same rows, us: norm 4096x3584 bf16 26.4 and
+ * 27.8, fp32 35.5 and 36.8; SwiGLU 512x18944 bf16 24.6 and 24.8, fp32 28.6 and
+ * 27.7.  Norm of rows that are not aligned 31.7. */
 template <template <typename, bool> class Row, typename T>
 cudaError_t launch_rows(const RowParams &p, int rows, int num_sms, cudaStream_t st) {
     const long long strides = p.a_stride | p.b_stride | (p.h != nullptr ? p.h_stride : 0);

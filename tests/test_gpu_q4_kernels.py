@@ -116,10 +116,10 @@ def test_matvec_kernel(kernel, shape, group, minimum):
     c.check(c.run(dtype), dtype)
 
 
-@pytest.mark.skipif(not torch.cuda.is_available() or torch.cuda.get_device_properties(0).multi_processor_count != 148,
-                    reason="the shapes are for 148 SMs")
 @pytest.mark.parametrize("kernel", sorted(SHAPES))
 def test_the_shapes_reach_their_kernels(kernel):
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("the shapes are for 148 SMs")
     for streams, rows, cols, pad in SHAPES[kernel]:
         for group in (32, 64, 128):
             c = Case(streams, rows, cols, group, False, pad=pad)
