@@ -103,9 +103,10 @@ template <typename T> union Four {
 /* Both directions: four lanes a block, a warp takes kRun runs of 256 columns of
  * a row, all their loads at once.  Bounded by HBM: 18944x3584 fp32 to 4 bits 53
  * us (0.88 of the measured rate; with minima and groups of 32 69), back 47.3
- * (0.99); bf16 60 us (108), bounded by instructions, and 32.  Of fp32, lane u of a block has columns 4u ..
- * 4u + 3 and 16 + 4u .., which are the word u; of 16-bit numbers eight columns
- * in a row, 16 bytes, and half a word's worth goes over to another lane. */
+ * (0.99); bf16 60 us (108), bounded by instructions, and 32.  Of fp32, lane u of
+ * a block has columns 4u .. 4u + 3 and 16 + 4u .., which are the word u; of 16-bit
+ * numbers eight columns in a row, 16 bytes, and half a word's worth goes over to
+ * another lane. */
 constexpr int kRun = 4;
 constexpr int kQ4Warps = 8;
 struct ConvertParams {
@@ -726,9 +727,9 @@ cudaError_t launch_mma(const MatvecParams &p, int x_base, int num_sms, cudaStrea
  * A CTA takes tiles of 128 rows by up to 64 streams.  The weights are the A
  * operand and lie in tensor memory: a thread of the eight unpacking warps has a
  * row, reads its 16-byte blocks from a ring of its warp's own (cp.async) and
- * stores 16 (q - 8), or with minima q, as int8, eight columns of tensor memory a block.  The
- * vectors are the B operand, in shared memory with the 128-byte swizzle.  One
- * thread issues the products, two groups of columns at a time into two of kTcD
+ * stores 16 (q - 8), or with minima q, as int8, eight columns of tensor memory a
+ * block.  The vectors are the B operand, in shared memory with the 128-byte
+ * swizzle.  One thread issues the products, two groups of columns at a time into two of kTcD
  * accumulators; sixteen warps read finished ones (int32, exact), scale them
  * by the row's scales of the groups and add them in fp32 registers, while the
  * next groups are multiplied.  So every scale is applied in fp32, the weights are
